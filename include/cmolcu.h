@@ -134,6 +134,81 @@ void cmolcu_matmul(float *out, const void *a, const float *b,
 void cmolcu_matmul_noalloc(float *out, const void *a, const float *b,
                            int m, int k, int n, int dtype);
 
+/* ---- 8-bit floating point: activations and weights in e4m3 ------------------
+ * No counterpart in the reference, whose formats are GGUF's.  A dense layer
+ * runs as a chain of three operators: cmolcu_fp8_rmsnorm (or _swiglu) leaves
+ * an activation in 8 bits, cmolcu_fp8_matmul multiplies it with weights that
+ * go to the tensor cores as they lie in memory.
+ *
+ * Format: e4m3 values in blocks with one f32 scale each; a value is q * scale.
+ * Activations have a block for every 128 consecutive values of a row, weights
+ * one for every 128 x 128 (a last block may be shorter).  The quantisers set
+ *   scale = max(amax / 448, 2^-126),   q = v / scale rounded to nearest even,
+ * so a block with a NaN gets a NaN scale and one with an infinity an infinite
+ * scale.
+ *
+ * Activations on the device: q is [n][k] bytes, k a multiple of 16, rows q_ld
+ * bytes apart; q starts on a 16-byte boundary and q_ld is a multiple of 16 (it
+ * does not count when n is 1).  The scale of (row c, block b) is at
+ * scales[c * s_ld + b * s_inc]: s_ld = 1, s_inc = n keeps the rows of a block
+ * together, which the wide products read best.  Bytes between the rows are
+ * neither read nor written.
+ *
+ * These calls only launch on `stream` (of `device`, or of the weight's
+ * device): they allocate nothing, use no workspace and can be captured.  The
+ * calling thread's current device is left as it was.  n = 0 does nothing.
+ * Outputs must not overlap inputs, but for res_out = res. */
+#define CMOLCU_BF16 30
+
+/* h = x + res (h = x when res is NULL); res_out = h rounded to res_dtype;
+ * v = norm_w[i] * (h[i] * 1/sqrt(mean(h^2) + eps)) from the unrounded h, or
+ * v = h when norm_w is NULL; q and scales of v.
+ * x, res, res_out: device rows of k values of CMOLCU_F32, _F16 or _BF16, x_ld
+ * / res_ld / res_out_ld values apart.  norm_w: k f32 values.  res_out may be
+ * res itself; both are NULL or neither.  Sums of squares are in f32. */
+int cmolcu_fp8_rmsnorm(int device, const void *x, int x_dtype, long long x_ld,
+                       const void *res, long long res_ld, void *res_out, long long res_out_ld, int res_dtype,
+                       const float *norm_w, float eps, int n, int k,
+                       void *q, long long q_ld, float *scales, long long s_ld, long long s_inc, void *stream);
+
+/* v = gate / (1 + exp(-gate)) * up; q and scales of v.  gate and up are rows
+ * of k values of `dtype`; both may be parts of one buffer (the product of the
+ * stacked gate and up weights: up = gate + k, both strides 2 k). */
+int cmolcu_fp8_swiglu(int device, const void *gate, long long gate_ld, const void *up, long long up_ld, int dtype,
+                      int n, int k,
+                      void *q, long long q_ld, float *scales, long long s_ld, long long s_inc, void *stream);
+
+/* A [rows x k] weight, laid out once for the product.
+ *   _upload       : q [rows][k] and scales [ceil(rows/128)][ceil(k/128)] on the host
+ *   _upload_dev   : the same on the device, rows q_ld bytes apart (q and q_ld
+ *                   multiples of 16), read on `stream`
+ *   _quantize_dev : from rows of `dtype` values on the device, ld values apart
+ *   _read_dev     : the weight's q (rows q_ld bytes apart) and scales, written
+ *                   to device memory on `stream`
+ * The three that make a weight allocate and wait for `stream`; they cannot be
+ * captured.  A weight can be used by any number of streams and threads at
+ * once.  Free it when no product that reads it is left to run. */
+typedef struct cmolcu_fp8_weight cmolcu_fp8_weight_t;
+int    cmolcu_fp8_weight_upload(int device, const void *q, const float *scales, int rows, int k,
+                                cmolcu_fp8_weight_t **out);
+int    cmolcu_fp8_weight_upload_dev(int device, const void *q, long long q_ld, const float *scales, int rows, int k,
+                                    void *stream, cmolcu_fp8_weight_t **out);
+int    cmolcu_fp8_weight_quantize_dev(int device, const void *w, int dtype, long long ld, int rows, int k,
+                                      void *stream, cmolcu_fp8_weight_t **out);
+int    cmolcu_fp8_weight_read_dev(const cmolcu_fp8_weight_t *w, void *q, long long q_ld, float *scales,
+                                  void *stream);
+void   cmolcu_fp8_weight_free(cmolcu_fp8_weight_t *w);
+size_t cmolcu_fp8_weight_bytes(const cmolcu_fp8_weight_t *w);   /* values and scales = bytes one pass reads */
+
+/* y(c, r) = sum_b sx(c, b) * sw(r/128, b) * sum_{k in b} qx(c, k) * qw(r, k) for
+ * n >= 1 activation rows: y is [n][rows] of y_dtype (CMOLCU_F32, _F16 or
+ * _BF16), y_ld values apart.  Products and sums in f32, one rounding at the
+ * end; the same call gives the same bits.  Waits inside the kernels are
+ * bounded (cmolcu_fault_status). */
+int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
+                      const float *scales, long long s_ld, long long s_inc, int n,
+                      void *y, int y_dtype, long long y_ld, void *stream);
+
 /* ---- host-only tokenizer -------------------------------------------------
  * The vocabulary of a GGUF file without loading weights or using a GPU:
  * the same encoder and decoder cmol_encode / cmol_decode_token use

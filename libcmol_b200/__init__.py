@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libcmol.so")
 
 # GGUF type tags
 F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 6, 8, 12, 14
+BF16 = 30
 
 _lib = None
 
@@ -72,6 +73,19 @@ def _declare(L):
     sig("cmolcu_fault_status", C.c_int, [C.c_int, C.POINTER(C.c_uint), C.c_int])
     sig("cmolcu_gemv_bench", C.c_int, [C.POINTER(_vp), C.c_int, _vp, C.c_int, _vp, C.c_int, C.c_int,
                                        C.POINTER(C.c_float)])
+    ll = C.c_longlong
+    sig("cmolcu_fp8_rmsnorm", C.c_int, [C.c_int, _vp, C.c_int, ll, _vp, ll, _vp, ll, C.c_int, _vp, C.c_float,
+                                        C.c_int, C.c_int, _vp, ll, _vp, ll, ll, _vp])
+    sig("cmolcu_fp8_swiglu", C.c_int, [C.c_int, _vp, ll, _vp, ll, C.c_int, C.c_int, C.c_int, _vp, ll, _vp, ll, ll,
+                                       _vp])
+    sig("cmolcu_fp8_weight_upload", C.c_int, [C.c_int, _vp, _vp, C.c_int, C.c_int, C.POINTER(_vp)])
+    sig("cmolcu_fp8_weight_upload_dev", C.c_int, [C.c_int, _vp, ll, _vp, C.c_int, C.c_int, _vp, C.POINTER(_vp)])
+    sig("cmolcu_fp8_weight_quantize_dev", C.c_int, [C.c_int, _vp, C.c_int, ll, C.c_int, C.c_int, _vp,
+                                                    C.POINTER(_vp)])
+    sig("cmolcu_fp8_weight_read_dev", C.c_int, [_vp, _vp, ll, _vp, _vp])
+    sig("cmolcu_fp8_weight_free", None, [_vp])
+    sig("cmolcu_fp8_weight_bytes", C.c_size_t, [_vp])
+    sig("cmolcu_fp8_matmul", C.c_int, [_vp, _vp, ll, _vp, ll, ll, C.c_int, _vp, C.c_int, ll, _vp])
     for name, res, args in _EXTRA_SIGS:
         if hasattr(L, name):
             sig(name, res, args)

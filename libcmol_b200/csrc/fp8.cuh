@@ -1,0 +1,128 @@
+// fp8.cuh — shared pieces of the 8-bit floating point path (cmolcu_fp8_*):
+// element types, e4m3 conversion, block scales, argument checks.
+//
+// A value v of a block is stored as q = rn_e4m3(v / s), s = max(amax / 448,
+// 2^-126), where amax is the block's largest magnitude: 448 is e4m3's largest
+// value, and the floor keeps 1 / s finite for blocks of zeros or of
+// subnormals.  A NaN in a block makes its scale NaN, an infinity makes the
+// scale infinite (and its own q NaN): either way every product with the block
+// is NaN or infinite, as it is without the rounding to 8 bits.
+#pragma once
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+
+#define FP8_BLOCK 128
+
+enum : int { DT_BF16 = 30 };          // GGUF numbering
+
+__host__ __device__ inline int fp8_blocks(int k) { return (k - 1) / FP8_BLOCK + 1; }
+
+// Bytes of an activation element, 0 for a type that the path does not take.
+inline int fp8_elem_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
+
+// Calls f with a value of the element type of tag `dt` (checked by the caller).
+template <typename F>
+auto fp8_with_type(int dt, F f) {
+    switch (dt) {
+    case DT_F16: return f(__half());
+    case DT_BF16: return f(__nv_bfloat16());
+    default: return f(float());
+    }
+}
+
+// The current device for the life of a call; the caller's is put back.
+struct Fp8Device {
+    int prev = -1;
+    cudaError_t err;
+    explicit Fp8Device(int dev) {
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && dev != prev) err = cudaSetDevice(dev);
+        else prev = -1;
+    }
+    ~Fp8Device() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+// Device fault word of the kernels behind cmolcu.h (seam.cu).
+unsigned int *cmolcu_fault_word(int device);
+
+// ---------------------------------------------------------------------------
+// Device: 8 values at a time
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float fp8_f(float v) { return v; }
+__device__ __forceinline__ float fp8_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float fp8_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T fp8_t(float v);
+template <>
+__device__ __forceinline__ float fp8_t<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half fp8_t<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 fp8_t<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight consecutive elements as they lie in memory: 16-byte accesses where
+// `vec` says that the address is 16-byte aligned, single elements otherwise.
+template <typename T>
+struct Fp8Oct {
+    T e[8];
+    __device__ __forceinline__ void load(const T *p, bool vec) {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(e) / 16; i++)
+                reinterpret_cast<uint4 *>(e)[i] = *(reinterpret_cast<const uint4 *>(p) + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) e[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void store(T *p, bool vec) const {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(e) / 16; i++)
+                *(reinterpret_cast<uint4 *>(p) + i) = reinterpret_cast<const uint4 *>(e)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[i] = e[i];
+        }
+    }
+};
+
+// max(a, |b|) that keeps a NaN of either side.
+__device__ __forceinline__ float fp8_amax(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+
+// Scale of a block from its largest magnitude.
+__device__ __forceinline__ float fp8_scale(float amax) {
+    const float s = __fdiv_rn(amax, 448.f), lo = 1.17549435e-38f;
+    return s < lo ? lo : s;           // a NaN passes
+}
+
+// Two e4m3 values, the first in the low byte (round to nearest even; a NaN
+// gives e4m3's NaN).
+__device__ __forceinline__ uint32_t fp8_pack2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint2 fp8_pack8(const float v[8], float inv) {
+    return make_uint2(fp8_pack2(v[0] * inv, v[1] * inv) | fp8_pack2(v[2] * inv, v[3] * inv) << 16,
+                      fp8_pack2(v[4] * inv, v[5] * inv) | fp8_pack2(v[6] * inv, v[7] * inv) << 16);
+}
+
+// Largest magnitude of the 128 values that 16 consecutive lanes hold, 8 each.
+__device__ __forceinline__ float fp8_amax16(const float v[8]) {
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a = fp8_amax(a, v[i]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a = fp8_amax(a, __shfl_xor_sync(0xffffffffu, a, o));
+    return a;
+}
