@@ -9,7 +9,10 @@
 #include "fp8_weight.cuh"
 #include "gemv_launch.cuh"
 
-#include <cuda_fp8.h>
+#include "tcgen05.cuh"
+
+#include <algorithm>
+#include <atomic>
 
 struct Fp8MmArgs {
     Fp8W           w;
@@ -22,31 +25,359 @@ struct Fp8MmArgs {
     long long      y_ld;
 };
 
-__device__ __forceinline__ float e4m3_f(uint8_t b) {
-    __nv_fp8_e4m3 v;
-    v.__x = b;
-    return (float)v;
+// ---------------------------------------------------------------------------
+// Few rows of activations: the weights' rows are the tensor core's M
+// ---------------------------------------------------------------------------
+// A CTA takes one row block of the weight (128 rows: the M of the product), NT
+// activation rows (its N) and a range of k blocks.  Every block of 128 along k
+// is a product of its own in tensor memory (four steps of K = 32); eight warps
+// take it from there, multiply by the block's scales and add to sums in
+// registers, while the tensor core forms the next blocks in other columns of
+// tensor memory.
+//
+// Bound by the weights' stream (one byte a value, read once per NT activation
+// rows): 16 KB blocks, contiguous along k, come by bulk copies into a ring.
+// Where the row blocks are fewer than the SMs, k is split over the CTAs of a
+// cluster, which add their sums through distributed shared memory in the
+// order of the split.
+//
+// Warps: 0 weights' producer, 1 tensor memory and products, 2 activations'
+// producer, 3 scales, 4-11 sums.
+#define MMN_THREADS 384
+#define MMN_SUM_WARPS 8
+#define MMN_SCALE_SLOTS 8
+#define MMN_MAX_STAGES 8
+
+struct Fp8MmnArgs {
+    CUtensorMap tm_q;          // activations: [n][k] bytes, box 128 x NT, 128-byte swizzle
+    Fp8MmArgs   a;
+    int         ksplit;        // CTAs of a cluster
+    int         kb_per;        // k blocks of a CTA
+    unsigned   *fault;
+};
+
+template <int NT>
+struct MmnCfg {
+    static constexpr int bufs = NT >= 128 ? 2 : 4;                        // products in tensor memory
+    static constexpr int cols = bufs * NT < 32 ? 32 : bufs * NT;
+    static constexpr int stage = FP8_TILE_BYTES + NT * FP8_BLOCK;
+    static constexpr int stages = (100 * 1024) / stage < MMN_MAX_STAGES ? (100 * 1024) / stage : MMN_MAX_STAGES;
+    static constexpr int smem = 1024 + stages * stage + MMN_SCALE_SLOTS * NT * 4;
+    static_assert(stages * stage >= NT * FP8_BLOCK * 4, "the sums of a CTA fit in its ring");
+};
+
+template <int NT, typename TY>
+__global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(const __grid_constant__ Fp8MmnArgs p) {
+    using Cfg = MmnCfg<NT>;
+    constexpr int S = Cfg::stages, B = Cfg::bufs, C = NT / 2;             // C: columns of a summing warp
+    const Fp8W &w = p.a.w;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const long long c0 = (long long)blockIdx.x * NT;                      // first activation row
+    const int ks = blockIdx.y, rb = blockIdx.z;
+    const int b0 = ks * p.kb_per, nb = min(w.kblocks - b0, p.kb_per);     // k blocks [b0, b0 + nb), nb >= 1
+    const int cols = (int)min((long long)NT, p.a.n - c0);
+
+    uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)cmolcu_smem + 1023) & ~(uintptr_t)1023);
+    float *scales = reinterpret_cast<float *>(base + S * Cfg::stage);     // [slot][NT]
+    __shared__ uint64_t full[S], empty[S], tfull[B], tempty[B], sfull[MMN_SCALE_SLOTS], sempty[MMN_SCALE_SLOTS], drain;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;                                               // a bounded wait ran out: every role gives up
+    volatile int *aborted = &s_abort;
+
+    if (tid == 0) {
+        t5_prefetch_map(&p.tm_q);
+        for (int i = 0; i < S; i++) {
+            mbar_init(&full[i], 2);                                       // both producers, with their bytes
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < B; i++) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], MMN_SUM_WARPS);
+        }
+        for (int i = 0; i < MMN_SCALE_SLOTS; i++) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&sempty[i], MMN_SUM_WARPS);
+        }
+        mbar_init(&drain, 1);
+        fence_mbar_init();
+        s_abort = 0;
+    }
+    if (warp == 1) t5_alloc(&s_tmem, Cfg::cols);
+    t5_fence_before();
+    __syncthreads();
+    t5_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_launch_dependents();
+
+    // A wait of a whole role: false when it, or another role's, ran out.
+    auto wait = [&](uint64_t *bar, int parity, unsigned code) {
+        if (!*aborted && mbar_wait(bar, parity, p.fault, code)) return true;
+        *aborted = 1;
+        return false;
+    };
+
+    uint64_t acc[C / 2];                                                  // sums of this lane's row, two columns each
+#pragma unroll
+    for (int i = 0; i < C / 2; i++) acc[i] = 0;
+
+    if (warp == 0 || warp == 2) {
+        // ---- producers: weights do not wait for the previous kernel, activations do ----
+        if (lane == 0) {
+            const bool wt = warp == 0;
+            if (!wt) pdl_wait();
+            const uint8_t *src = w.tiles + ((size_t)rb * w.kblocks + b0) * FP8_TILE_BYTES;
+            int i = 0;
+            for (; i < nb; i++) {
+                const int st = i % S, use = i / S;
+                if (use > 0 && !wait(&empty[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) break;
+                uint8_t *dst = base + st * Cfg::stage;
+                if (wt) {
+                    mbar_arrive_expect_tx(&full[st], FP8_TILE_BYTES);
+                    bulk_g2s(dst, src + (size_t)i * FP8_TILE_BYTES, FP8_TILE_BYTES, &full[st]);
+                } else {
+                    mbar_arrive_expect_tx(&full[st], NT * FP8_BLOCK);
+                    t5_tma_2d(dst + FP8_TILE_BYTES, &p.tm_q, (b0 + i) * FP8_BLOCK, (int)c0, &full[st]);
+                }
+            }
+            if (*aborted)                                                 // what was issued lands before the CTA ends
+                for (int j = max(0, i - S); j < i; j++) mbar_wait(&full[j % S], (j / S) & 1, nullptr, 0);
+        }
+    } else if (warp == 1) {
+        // ---- products ----
+        if (lane == 0) {
+            const uint32_t idesc = t5_idesc_e4m3(FP8_BLOCK, NT);
+            for (int i = 0; i < nb; i++) {
+                const int st = i % S, tb = i % B;
+                if (i >= B && !wait(&tempty[tb], (i / B - 1) & 1, FAULT_GEMV_EMPTY)) break;
+                if (!wait(&full[st], (i / S) & 1, FAULT_GEMV_FULL)) break;
+                t5_fence_after();
+                const uint32_t sa = smem_u32(base + st * Cfg::stage), sb = sa + FP8_TILE_BYTES;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    t5_mma_e4m3(tmem + tb * NT, t5_desc(sa + 32 * k), t5_desc(sb + 32 * k), idesc, k > 0);
+                t5_commit(&empty[st]);
+                t5_commit(&tfull[tb]);
+            }
+            t5_commit(&drain);
+            mbar_wait(&drain, 0, p.fault, FAULT_GEMV_FULL);
+        }
+    } else if (warp == 3) {
+        // ---- scales: activation scale x weight scale, four blocks' loads in flight ----
+        constexpr int L = (NT + 31) / 32;
+        pdl_wait();
+        const float *sw = w.scales + (size_t)rb * w.kblocks + b0;
+        for (int i0 = 0; i0 < nb; i0 += 4) {
+            float v[4][L];
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int l = 0; l < L; l++) {
+                    const int c = l * 32 + lane;
+                    v[g][l] = i0 + g < nb && c < cols
+                                  ? p.a.s[(c0 + c) * p.a.s_ld + (long long)(b0 + i0 + g) * p.a.s_inc] * sw[i0 + g]
+                                  : 0.f;
+                }
+            bool ok = true;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int i = i0 + g, sl = i % MMN_SCALE_SLOTS;
+                if (i >= nb) break;
+                ok = ok && (i < MMN_SCALE_SLOTS ||
+                            __all_sync(0xffffffffu, wait(&sempty[sl], (i / MMN_SCALE_SLOTS - 1) & 1, FAULT_GEMV_EMPTY)));
+                if (!ok) break;
+#pragma unroll
+                for (int l = 0; l < L; l++)
+                    if (l * 32 + lane < NT) scales[sl * NT + l * 32 + lane] = v[g][l];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfull[sl]);
+            }
+            if (!ok) break;
+        }
+    } else {
+        // ---- sums: warp w has tensor-memory lanes 32 * (w % 4) .., half of the columns ----
+        const int half = (warp - 4) >> 2;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        for (int i = 0; i < nb; i++) {
+            const int tb = i % B, sl = i % MMN_SCALE_SLOTS;
+            const bool ok = wait(&tfull[tb], (i / B) & 1, FAULT_GEMV_FULL) &&
+                            wait(&sfull[sl], (i / MMN_SCALE_SLOTS) & 1, FAULT_GEMV_FULL);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            t5_fence_after();
+            const float *sc = scales + sl * NT + half * C;
+            constexpr int W = C < 32 ? C : 32;
+#pragma unroll
+            for (int j0 = 0; j0 < C; j0 += W) {
+                uint32_t d[W];
+                t5_ld(tmem + lanes + tb * NT + half * C + j0, d);
+                t5_wait_ld(d);
+#pragma unroll
+                for (int j = 0; j < W; j += 4) {
+                    const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(sc + j0 + j);
+                    acc[(j0 + j) / 2] = t5_fma2(t5_pair(d[j], d[j + 1]), s4.x, acc[(j0 + j) / 2]);
+                    acc[(j0 + j) / 2 + 1] = t5_fma2(t5_pair(d[j + 2], d[j + 3]), s4.y, acc[(j0 + j) / 2 + 1]);
+                }
+            }
+            t5_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&tempty[tb]);
+                mbar_arrive(&sempty[sl]);
+            }
+        }
+    }
+    __syncwarp();
+    __syncthreads();                                                      // the ring is drained: every product is done
+
+    TY *y = static_cast<TY *>(p.a.y);
+    const int r0 = rb * FP8_BLOCK;
+    if (warp >= 4) {
+        const int half = (warp - 4) >> 2, r = 32 * (warp & 3) + lane;
+        if (p.ksplit == 1) {
+            pdl_wait();
+            TY *yr = y + (c0 + half * C) * p.a.y_ld + r0 + r;
+#pragma unroll
+            for (int i = 0; i < C / 2; i++) {
+                float v0, v1;
+                t5_unpair(acc[i], v0, v1);
+                if (r0 + r < w.rows) {
+                    if (half * C + 2 * i < cols) yr[(long long)(2 * i) * p.a.y_ld] = fp8_t<TY>(v0);
+                    if (half * C + 2 * i + 1 < cols) yr[(long long)(2 * i + 1) * p.a.y_ld] = fp8_t<TY>(v1);
+                }
+            }
+        } else {
+            float *part = reinterpret_cast<float *>(base) + (half * C) * FP8_BLOCK + r;
+#pragma unroll
+            for (int i = 0; i < C / 2; i++) t5_unpair(acc[i], part[2 * i * FP8_BLOCK], part[(2 * i + 1) * FP8_BLOCK]);
+        }
+    }
+    if (p.ksplit > 1) {
+        // task = (column, 4 rows), dealt over the threads of the cluster's CTAs
+        t5_cluster_sync();
+        pdl_wait();
+        const uint32_t part = smem_u32(base);
+        for (int t = ks * MMN_THREADS + tid; t < cols * 32; t += p.ksplit * MMN_THREADS) {
+            const int col = t >> 5, rq = (t & 31) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < p.ksplit; s++) {
+                const float4 u = t5_cluster_ld4(t5_cluster_addr(part + (col * FP8_BLOCK + rq) * 4, s));
+                v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+            }
+            TY *yc = y + (c0 + col) * p.a.y_ld + r0 + rq;
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (r0 + rq + j < w.rows) yc[j] = fp8_t<TY>(e[j]);
+        }
+        t5_cluster_sync();                                                // the sums stay until every CTA has read them
+    }
+    if (warp == 1) {
+        t5_fence_after();
+        t5_dealloc(tmem, Cfg::cols);
+    }
 }
 
-// One thread a value of y, 16 columns x 16 rows a CTA: every product formed
-// in f32.
-template <typename TY>
-__global__ void __launch_bounds__(256) k_fp8_mm_simple(const Fp8MmArgs a) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int r = blockIdx.x * 16 + (threadIdx.x & 15);
-    const long long c = (long long)blockIdx.y * 16 + (threadIdx.x >> 4);
-    if (r >= a.w.rows || c >= a.n) return;
-    float acc = 0.f;
-    for (int b = 0; b < a.w.kblocks; b++) {
-        const uint8_t *t = a.w.tiles + ((size_t)(r >> 7) * a.w.kblocks + b) * FP8_TILE_BYTES;
-        const uint8_t *x = a.q + c * a.q_ld + (long long)b * FP8_BLOCK;
-        const int len = min(FP8_BLOCK, a.w.k - b * FP8_BLOCK);
-        float d = 0.f;
-        for (int k = 0; k < len; k++) d = __fmaf_rn(e4m3_f(x[k]), e4m3_f(t[fp8_tile_byte(r & 127, k)]), d);
-        acc = __fmaf_rn(d, a.s[c * a.s_ld + b * a.s_inc] * a.w.scales[(size_t)(r >> 7) * a.w.kblocks + b], acc);
-    }
-    static_cast<TY *>(a.y)[c * a.y_ld + r] = fp8_t<TY>(acc);
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+// cuTensorMapEncodeTiled, reached through the runtime's driver entry point (no
+// link-time dependency on the driver library).
+typedef CUresult (*encode_t)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static encode_t encode_fn() {
+    static const encode_t fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<encode_t>(f);
+    }();
+    return fn;
+}
+
+// Activations as [n][k] bytes, read in boxes of `rows` rows x 128 bytes with
+// the 128-byte swizzle; what lies past n or k reads as zero.
+static bool q_map(CUtensorMap *m, const Fp8MmArgs &a, int rows) {
+    const encode_t enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.w.k, (cuuint64_t)a.n};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.q_ld};
+    const cuuint32_t box[2] = {FP8_BLOCK, (cuuint32_t)rows}, es[2] = {1u, 1u};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(a.q), dims, strides, box, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Launch with programmatic dependent launch and a (1, cluster, 1) cluster.
+template <typename P>
+static cudaError_t mm_launch(void (*k)(P), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
+                             const P &p) {
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 1;
+    at[1].val.clusterDim.y = cluster;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, p);
+}
+
+// Largest cluster (16, else the portable 8) in which kernel k runs on the
+// current device.
+template <typename P>
+static int max_cluster(void (*k)(P), int threads, size_t smem) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, 16);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 1;
+    at.val.clusterDim.y = 16;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const bool ok =
+        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
+        cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0;
+    cudaGetLastError();                 // a refused query leaves no error behind
+    return ok ? 16 : 8;
+}
+
+template <int NT, typename TY>
+static cudaError_t mmn_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
+    using Cfg = MmnCfg<NT>;
+    Fp8MmnArgs p = {};
+    p.a = a;
+    p.fault = fault;
+    if (!q_map(&p.tm_q, a, NT)) return cudaErrorInvalidValue;
+    const long long tiles = (a.n - 1) / NT + 1;
+    // as many CTAs a row block as fill one wave, at least one k block each
+    static std::atomic<int> cluster[64];                                 // per device, 0: not asked yet
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!cluster[dev]) cluster[dev] = max_cluster(k_fp8_mm_n<NT, TY>, MMN_THREADS, Cfg::smem);
+    const int slots = device_sm_count() * (NT <= 64 ? 2 : 1);
+    int ks = (int)std::max<long long>(1, std::min<long long>(std::min<int>(cluster[dev], a.w.kblocks), slots / (tiles * a.w.rblocks)));
+    p.kb_per = (a.w.kblocks + ks - 1) / ks;
+    p.ksplit = (a.w.kblocks + p.kb_per - 1) / p.kb_per;
+    const dim3 grid((unsigned)tiles, p.ksplit, a.w.rblocks);
+    return mm_launch(k_fp8_mm_n<NT, TY>, grid, MMN_THREADS, Cfg::smem, p.ksplit, st, p);
 }
 
 extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld, const float *scales,
@@ -71,9 +402,14 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
     a.q = static_cast<const uint8_t *>(q); a.q_ld = q_ld;
     a.s = scales; a.s_ld = s_ld; a.s_inc = s_inc;
     a.n = n; a.y = y; a.y_ld = y_ld;
-    const dim3 grid((a.w.rows + 15) / 16, (n + 15) / 16);
+    unsigned *fault = cmolcu_fault_word(w->device);
+    const cudaStream_t st = (cudaStream_t)stream;
     CUDA_TRY(fp8_with_type(y_dtype, [&](auto t) {
-        return launch_k(k_fp8_mm_simple<decltype(t)>, grid, dim3(256), 0, (cudaStream_t)stream, true, a);
+        using TY = decltype(t);
+        if (n <= 16) return mmn_launch<16, TY>(a, fault, st);
+        if (n <= 32) return mmn_launch<32, TY>(a, fault, st);
+        if (n <= 64) return mmn_launch<64, TY>(a, fault, st);
+        return mmn_launch<128, TY>(a, fault, st);
     }));
     return 0;
 }
