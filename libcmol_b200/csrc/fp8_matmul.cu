@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
 
     // A wait of a whole role: false when it, or another role's, ran out.
     auto wait = [&](uint64_t *bar, int parity, unsigned code) {
+        if (mbar_try_wait(bar, parity)) return true;
         if (!*aborted && mbar_wait(bar, parity, p.fault, code)) return true;
         *aborted = 1;
         return false;
@@ -124,11 +125,12 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
         // ---- producers: weights do not wait for the previous kernel, activations do ----
         if (lane == 0) {
             const bool wt = warp == 0;
-            if (!wt) pdl_wait();
+            if (!wt) pdl_wait();                                          // (nor does any bounded wait span it)
             const uint8_t *src = w.tiles + ((size_t)rb * w.kblocks + b0) * FP8_TILE_BYTES;
             int i = 0;
             for (; i < nb; i++) {
                 const int st = i % S, use = i / S;
+                if (i == S) pdl_wait();
                 if (use > 0 && !wait(&empty[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) break;
                 uint8_t *dst = base + st * Cfg::stage;
                 if (wt) {
@@ -144,6 +146,7 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
         }
     } else if (warp == 1) {
         // ---- products ----
+        pdl_wait();
         if (lane == 0) {
             const uint32_t idesc = t5_idesc_e4m3(FP8_BLOCK, NT);
             for (int i = 0; i < nb; i++) {
@@ -195,6 +198,7 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
         }
     } else {
         // ---- sums: warp w has tensor-memory lanes 32 * (w % 4) .., half of the columns ----
+        pdl_wait();
         const int half = (warp - 4) >> 2;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         for (int i = 0; i < nb; i++) {
@@ -233,7 +237,6 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
     if (warp >= 4) {
         const int half = (warp - 4) >> 2, r = 32 * (warp & 3) + lane;
         if (p.ksplit == 1) {
-            pdl_wait();
             TY *yr = y + (c0 + half * C) * p.a.y_ld + r0 + r;
 #pragma unroll
             for (int i = 0; i < C / 2; i++) {
@@ -273,6 +276,241 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
     if (warp == 1) {
         t5_fence_after();
         t5_dealloc(tmem, Cfg::cols);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows of activations: they are the tensor core's M
+// ---------------------------------------------------------------------------
+// Two CTAs (a cluster on neighbouring SMs) form one tile of 256 activation rows
+// x 256 weight rows: each holds 128 of both in shared memory, and every product
+// of the pair (M = N = 256) reads both halves, so an SM loads 32 KB a block of
+// 128 along k for work that takes its tensor core 512 clocks.  A lane of
+// tensor memory is an activation row here and a warp's 128 columns are one
+// row block of the weight, so a block's scale is one number a thread: taking a
+// block's product from tensor memory and adding it (128 columns a thread, two
+// values an instruction) measured ~300 clocks an SM, which hides behind the
+// products, as the double buffer in tensor memory lets both run at once.
+// (With the roles of the operands as in k_fp8_mm_n the scale differs from column
+// to column and comes from shared memory: 670 clocks.)
+//
+// The CTAs are persistent: loads and products run on into the next tile while
+// the sums of the last are written.
+//
+// Warps: 0 loads, 1 products (rank 0), 2 tensor memory, 4-11 sums.
+#define MMT_THREADS 384
+#define MMT_STAGES 6
+#define MMT_STAGE (2 * FP8_TILE_BYTES)
+#define MMT_STAGING (8 * 32 * 128)          // a summing warp's way out: 32 rows x 128 bytes
+#define MMT_SMEM (1024 + MMT_STAGES * MMT_STAGE + MMT_STAGING)
+// Registers: 168 a thread at launch; the sums hold 128 of them and what tensor
+// memory gives, the other warps need few.  128 * 56 + 256 * 224 = 384 * 168.
+#define MMT_REGS 168
+#define MMT_REGS_FEW 56
+#define MMT_REGS_SUMS 224
+static_assert(128 * MMT_REGS_FEW + 256 * MMT_REGS_SUMS == MMT_THREADS * MMT_REGS, "register split");
+
+struct Fp8MmtArgs {
+    CUtensorMap tm_q, tm_w;    // activations as above; weight tiles as rows of 128 bytes
+    Fp8MmArgs   a;
+    int         mt, rt;        // tiles of activation rows and of weight rows
+    int         vy;            // rows of y start on 16-byte boundaries
+    unsigned   *fault;
+};
+
+template <typename TY>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp8_mm_t(const __grid_constant__ Fp8MmtArgs p) {
+    constexpr int S = MMT_STAGES;
+    const Fp8W &w = p.a.w;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)t5_cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const long long tiles = (long long)p.mt * p.rt;
+    const int nb = w.kblocks;
+
+    uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)cmolcu_smem + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[S], empty[S], tfull[2], tempty[2], drain;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    volatile int *aborted = &s_abort;
+
+    if (tid == 0) {
+        t5_prefetch_map(&p.tm_q);
+        t5_prefetch_map(&p.tm_w);
+        for (int i = 0; i < S; i++) {
+            mbar_init(&full[i], 1);             // rank 0's, for the bytes of both
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], 16);          // rank 0's, for the summing warps of both
+        }
+        mbar_init(&drain, 1);
+        fence_mbar_init();
+        s_abort = 0;
+    }
+    if (warp == 2) t5_alloc2(&s_tmem, 512);
+    t5_fence_before();
+    __syncthreads();
+    t5_cluster_sync();                          // the other CTA's barriers are there
+    t5_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_launch_dependents();
+
+    auto wait = [&](uint64_t *bar, int parity, unsigned code) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (!*aborted && mbar_wait(bar, parity, p.fault, code)) return true;
+        *aborted = 1;
+        return false;
+    };
+
+    if (warp < 4) {
+        t5_regs_dec<MMT_REGS_FEW>();
+        if (warp == 0 && lane == 0) {
+            // ---- loads: this CTA's halves, counted on rank 0's barriers ----
+            pdl_wait();
+            int st = 0, use = 0;
+            bool ok = true;
+            for (long long t = pair; t < tiles && ok; t += pairs) {
+                const int m = (int)(t % p.mt), r = (int)(t / p.mt);
+                const int row = m * 256 + rank * 128, rb = 2 * r + rank;
+                for (int i = 0; i < nb; i++) {
+                    if (use > 0 && !wait(&empty[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *dst = base + st * MMT_STAGE;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * MMT_STAGE);
+                    const uint32_t bar = t5_cluster_addr(smem_u32(&full[st]), 0);
+                    t5_tma2_2d(dst, &p.tm_q, i * FP8_BLOCK, row, bar);
+                    t5_tma2_2d(dst + FP8_TILE_BYTES, &p.tm_w, 0, (rb * nb + i) * FP8_BLOCK, bar);
+                    if (++st == S) { st = 0; use++; }
+                }
+            }
+            if (!ok && rank == 0)               // what was issued lands before the cluster ends
+                for (int j = 0; j < S; j++) {
+                    const int u = j < st ? use : use - 1;
+                    if (u >= 0) mbar_wait(&full[j], u & 1, nullptr, 0);
+                }
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            // ---- products ----
+            pdl_wait();                         // so that no bounded wait spans the previous kernel
+            const uint32_t idesc = t5_idesc_e4m3(256, 256);
+            int st = 0, use = 0, tb = 0, tuse = 0;
+            bool ok = true;
+            for (long long t = pair; t < tiles && ok; t += pairs)
+                for (int i = 0; i < nb; i++) {
+                    ok = (tuse == 0 || wait(&tempty[tb], (tuse - 1) & 1, FAULT_GEMV_EMPTY)) &&
+                         wait(&full[st], use & 1, FAULT_GEMV_FULL);
+                    if (!ok) break;
+                    t5_fence_after();
+                    const uint32_t sa = smem_u32(base + st * MMT_STAGE), sb = sa + FP8_TILE_BYTES;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        t5_mma2_e4m3(tmem + tb * 256, t5_desc(sa + 32 * k), t5_desc(sb + 32 * k), idesc, k > 0);
+                    t5_commit2(&empty[st]);
+                    t5_commit2(&tfull[tb]);
+                    if (++st == S) { st = 0; use++; }
+                    if (++tb == 2) { tb = 0; tuse++; }
+                }
+            t5_commit2(&drain);
+        }
+    } else {
+        // ---- sums: lanes 32 * (warp % 4) .. are activation rows, 128 columns one row block ----
+        t5_regs_inc<MMT_REGS_SUMS>();
+        pdl_wait();
+        const int half = (warp - 4) >> 2, lrow = rank * 128 + 32 * (warp & 3);
+        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 128;
+        uint8_t *stg = base + S * MMT_STAGE + (warp - 4) * (32 * 128);
+        int tb = 0, tuse = 0;
+        bool ok = true;
+        for (long long t = pair; t < tiles && ok; t += pairs) {
+            const int m = (int)(t % p.mt), r = (int)(t / p.mt);
+            const long long row = (long long)m * 256 + lrow + lane;      // this lane's activation row
+            const int rb = 2 * r + half;
+            const bool live = row < p.a.n && rb < w.rblocks;
+            const float *sx = p.a.s + row * p.a.s_ld, *sw = w.scales + (size_t)rb * nb;
+            uint64_t acc[64];
+#pragma unroll
+            for (int j = 0; j < 64; j++) acc[j] = 0;
+            float x1 = live ? sx[0] : 0.f, w1 = live ? sw[0] : 0.f;
+            for (int i = 0; i < nb; i++) {
+                const float s = x1 * w1;
+                const uint64_t s2 = t5_pair(__float_as_uint(s), __float_as_uint(s));
+                if (live && i + 1 < nb) {                                 // the next block's, while this one is added
+                    x1 = sx[(long long)(i + 1) * p.a.s_inc];
+                    w1 = sw[i + 1];
+                }
+                ok = __all_sync(0xffffffffu, wait(&tfull[tb], tuse & 1, FAULT_GEMV_FULL));
+                if (!ok) break;
+                t5_fence_after();
+                uint32_t d[2][32];
+                t5_ld(tcol + tb * 256, d[0]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    t5_wait_ld(d[c & 1]);
+                    if (c < 3) t5_ld(tcol + tb * 256 + 32 * (c + 1), d[(c + 1) & 1]);
+                    else {
+                        t5_fence_before();
+                        __syncwarp();
+                        if (lane == 0) t5_cluster_arrive(t5_cluster_addr(smem_u32(&tempty[tb]), 0));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        acc[c * 16 + j] = t5_fma2(t5_pair(d[c & 1][2 * j], d[c & 1][2 * j + 1]), s2, acc[c * 16 + j]);
+                }
+                if (++tb == 2) { tb = 0; tuse++; }
+            }
+            if (!ok || rb >= w.rblocks) continue;
+            // ---- out: 128 bytes of each of the warp's 32 rows at a time, through shared memory ----
+            constexpr int E = 128 / sizeof(TY), V = 16 / sizeof(TY);      // columns a pass, columns a 16-byte chunk
+            TY *y = static_cast<TY *>(p.a.y);
+#pragma unroll
+            for (int ps = 0; ps < 128 / E; ps++) {
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    TY v[V];
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        float lo, hi;
+                        t5_unpair(acc[(ps * E + c * V + e) / 2], lo, hi);
+                        v[e] = fp8_t<TY>(lo);
+                        v[e + 1] = fp8_t<TY>(hi);
+                    }
+                    *reinterpret_cast<uint4 *>(stg + lane * 128 + ((c ^ (lane & 7)) << 4)) = *reinterpret_cast<uint4 *>(v);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int it = 0; it < 8; it++) {
+                    const int lr = it * 4 + (lane >> 3), ch = lane & 7;
+                    const long long orow = (long long)m * 256 + lrow + lr;
+                    const int ocol = rb * FP8_BLOCK + ps * E + ch * V;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stg + lr * 128 + ((ch ^ (lr & 7)) << 4));
+                    if (orow < p.a.n) {
+                        TY *o = y + orow * p.a.y_ld + ocol;
+                        if (p.vy && ocol + V <= w.rows) {
+                            *reinterpret_cast<uint4 *>(o) = v;
+                        } else {
+                            const TY *e = reinterpret_cast<const TY *>(&v);
+#pragma unroll
+                            for (int j = 0; j < V; j++)
+                                if (ocol + j < w.rows) o[j] = e[j];
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+    t5_fence_before();
+    __syncthreads();
+    if (tid == 0) mbar_wait(&drain, 0, p.fault, FAULT_GEMV_FULL);        // the last arrival from rank 0's products
+    __syncwarp();
+    t5_cluster_sync();                          // neither CTA's memory is in use by the other any more
+    if (warp == 2) {
+        t5_fence_after();
+        t5_dealloc2(tmem, 512);
     }
 }
 
@@ -380,12 +618,53 @@ static cudaError_t mmn_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     return mm_launch(k_fp8_mm_n<NT, TY>, grid, MMN_THREADS, Cfg::smem, p.ksplit, st, p);
 }
 
+// Weight tiles as rows of 128 bytes, read a tile at a time (their bytes are in
+// the operand's swizzled order already); row blocks past the last read as zero.
+static bool w_map(CUtensorMap *m, const Fp8W &w) {
+    const encode_t enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {FP8_BLOCK, (cuuint64_t)w.rblocks * w.kblocks * FP8_BLOCK};
+    const cuuint64_t strides[1] = {FP8_BLOCK};
+    const cuuint32_t box[2] = {FP8_BLOCK, FP8_BLOCK}, es[2] = {1u, 1u};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(w.tiles), dims, strides, box, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename TY>
+static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
+    const auto kern = k_fp8_mm_t<TY>;
+    Fp8MmtArgs p = {};
+    p.a = a;
+    p.fault = fault;
+    if (!q_map(&p.tm_q, a, FP8_BLOCK) || !w_map(&p.tm_w, a.w)) return cudaErrorInvalidValue;
+    p.mt = (a.n - 1) / 256 + 1;
+    p.rt = (a.w.rblocks - 1) / 2 + 1;
+    p.vy = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.n == 1 || (a.y_ld * sizeof(TY)) % 16 == 0);
+    // the register split of the kernel adds up only to what it was built with
+    static std::atomic<int> ready[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!ready[dev]) {
+        cudaFuncAttributes fa = {};
+        cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+        if (e == cudaSuccess && fa.numRegs != MMT_REGS) e = cudaErrorInvalidConfiguration;
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MMT_SMEM);
+        if (e != cudaSuccess) return e;
+        ready[dev] = 1;
+    }
+    const long long tiles = (long long)p.mt * p.rt;
+    const int pairs = (int)std::min<long long>(tiles, device_sm_count() / 2);
+    return launch_k(kern, dim3(2 * pairs), dim3(MMT_THREADS), MMT_SMEM, st, true, p);
+}
+
 extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld, const float *scales,
                                  long long s_ld, long long s_inc, int n, void *y, int y_dtype, long long y_ld,
                                  void *stream) {
     static const char *who = "cmolcu_fp8_matmul";
     if (!w) { cmolcu_set_error("%s: NULL argument", who); return -1; }
-    if (n < 0) { cmolcu_set_error("%s: n=%d", who, n); return -1; }
+    if (n < 0 || n > 1 << 30) { cmolcu_set_error("%s: n=%d", who, n); return -1; }
     if (!fp8_elem_bytes(y_dtype)) { cmolcu_set_error("%s: unsupported dtype %d", who, y_dtype); return -1; }
     if (n == 0) return 0;
     if (!q || !scales || !y) { cmolcu_set_error("%s: NULL argument", who); return -1; }
@@ -409,7 +688,8 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
         if (n <= 16) return mmn_launch<16, TY>(a, fault, st);
         if (n <= 32) return mmn_launch<32, TY>(a, fault, st);
         if (n <= 64) return mmn_launch<64, TY>(a, fault, st);
-        return mmn_launch<128, TY>(a, fault, st);
+        if (n <= 128) return mmn_launch<128, TY>(a, fault, st);
+        return mmt_launch<TY>(a, fault, st);
     }));
     return 0;
 }
