@@ -397,21 +397,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             pdl_wait();                         // so that no bounded wait spans the previous kernel
             const uint32_t idesc = t5_idesc_e4m3(256, 256);
             int st = 0, use = 0, tb = 0, tuse = 0;
-            bool ok = true;
+            bool ok = true, ready = false;      // ready: the barriers of this block were seen complete in the last
             for (long long t = pair; t < tiles && ok; t += pairs)
                 for (int i = 0; i < nb; i++) {
-                    ok = (tuse == 0 || wait(&tempty[tb], (tuse - 1) & 1, FAULT_GEMV_EMPTY)) &&
-                         wait(&full[st], use & 1, FAULT_GEMV_FULL);
+                    ok = ready || ((tuse == 0 || wait(&tempty[tb], (tuse - 1) & 1, FAULT_GEMV_EMPTY)) &&
+                                   wait(&full[st], use & 1, FAULT_GEMV_FULL));
                     if (!ok) break;
                     t5_fence_after();
-                    const uint32_t sa = smem_u32(base + st * MMT_STAGE), sb = sa + FP8_TILE_BYTES;
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        t5_mma2_e4m3(tmem + tb * 256, t5_desc(sa + 32 * k), t5_desc(sb + 32 * k), idesc, k > 0);
-                    t5_commit2(&empty[st]);
-                    t5_commit2(&tfull[tb]);
+                    const uint32_t sa = smem_u32(base + st * MMT_STAGE), sb = sa + FP8_TILE_BYTES, d = tmem + tb * 256;
+                    uint64_t *const e = &empty[st], *const f = &tfull[tb];
                     if (++st == S) { st = 0; use++; }
                     if (++tb == 2) { tb = 0; tuse++; }
+                    const bool r0 = tuse == 0 || mbar_test(&tempty[tb], (tuse - 1) & 1);
+                    const bool r1 = mbar_test(&full[st], use & 1);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        t5_mma2_e4m3(d, t5_desc(sa + 32 * k), t5_desc(sb + 32 * k), idesc, k > 0);
+                    t5_commit2(e);
+                    t5_commit2(f);
+                    ready = r0 && r1;
                 }
             t5_commit2(&drain);
         }
