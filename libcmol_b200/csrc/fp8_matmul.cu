@@ -297,18 +297,26 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
 // The CTAs are persistent: loads and products run on into the next tile while
 // the sums of the last are written.
 //
-// Warps: 0 loads, 1 products (rank 0), 2 tensor memory, 4-11 sums.
-#define MMT_THREADS 384
+// A wait or an arrival costs a thread about as much as two products cost it to
+// issue, so two warps issue in turn (the two halves of tensor memory), and there
+// are two barriers a block: `full` counts the bytes of both
+// CTAs' stages and the 32 summing warps' release of the half of tensor memory
+// that the block will use, `done` (the products' commit, in both CTAs) frees
+// the stage and hands the sums their block.
+//
+// Warps: 0 loads, 1 and 3 products (rank 0), 2 tensor memory, 4-19 sums (four a
+// scheduler: with two, the time that each spends on barriers showed).
+#define MMT_SUM_WARPS 16
+#define MMT_THREADS (128 + 32 * MMT_SUM_WARPS)
 #define MMT_STAGES 6
 #define MMT_STAGE (2 * FP8_TILE_BYTES)
-#define MMT_STAGING (8 * 32 * 128)          // a summing warp's way out: 32 rows x 128 bytes
+#define MMT_STAGING (MMT_SUM_WARPS * 32 * 64)       // a summing warp's way out: 32 rows x 64 bytes
 #define MMT_SMEM (1024 + MMT_STAGES * MMT_STAGE + MMT_STAGING)
-// Registers: 168 a thread at launch; the sums hold 128 of them and what tensor
-// memory gives, the other warps need few.  128 * 56 + 256 * 224 = 384 * 168.
-#define MMT_REGS 168
-#define MMT_REGS_FEW 56
-#define MMT_REGS_SUMS 224
-static_assert(128 * MMT_REGS_FEW + 256 * MMT_REGS_SUMS == MMT_THREADS * MMT_REGS, "register split");
+// Registers a thread at launch, of the first warpgroup and of the summing warps.
+#define MMT_REGS 96
+#define MMT_REGS_FEW 64
+#define MMT_REGS_SUMS 104
+static_assert(128 * MMT_REGS_FEW + 32 * MMT_SUM_WARPS * MMT_REGS_SUMS == MMT_THREADS * MMT_REGS, "register split");
 
 struct Fp8MmtArgs {
     CUtensorMap tm_q, tm_w;    // activations as above; weight tiles as rows of 128 bytes
@@ -321,6 +329,7 @@ struct Fp8MmtArgs {
 template <typename TY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp8_mm_t(const __grid_constant__ Fp8MmtArgs p) {
     constexpr int S = MMT_STAGES;
+    static_assert(S % 2 == 0 && S >= 4, "a stage belongs to one half of tensor memory");
     const Fp8W &w = p.a.w;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)t5_cluster_rank();
@@ -329,7 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
     const int nb = w.kblocks;
 
     uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)cmolcu_smem + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[S], empty[S], tfull[2], tempty[2], drain;
+    __shared__ uint64_t full[S], done[S], drain;        // full: rank 0's counts
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     volatile int *aborted = &s_abort;
@@ -338,14 +347,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
         t5_prefetch_map(&p.tm_q);
         t5_prefetch_map(&p.tm_w);
         for (int i = 0; i < S; i++) {
-            mbar_init(&full[i], 1);             // rank 0's, for the bytes of both
-            mbar_init(&empty[i], 1);
+            mbar_init(&full[i], 1 + 2 * MMT_SUM_WARPS);
+            mbar_init(&done[i], 1);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], 16);          // rank 0's, for the summing warps of both
-        }
-        mbar_init(&drain, 1);
+        mbar_init(&drain, 2);
         fence_mbar_init();
         s_abort = 0;
     }
@@ -375,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                 const int m = (int)(t % p.mt), r = (int)(t / p.mt);
                 const int row = m * 256 + rank * 128, rb = 2 * r + rank;
                 for (int i = 0; i < nb; i++) {
-                    if (use > 0 && !wait(&empty[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) {
+                    if (use > 0 && !wait(&done[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) {
                         ok = false;
                         break;
                     }
@@ -392,87 +397,95 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                     const int u = j < st ? use : use - 1;
                     if (u >= 0) mbar_wait(&full[j], u & 1, nullptr, 0);
                 }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
-            // ---- products ----
+        } else if ((warp & 1) && lane == 0 && rank == 0) {
+            // ---- products: warp 1 the even blocks, warp 3 the odd ones ----
             pdl_wait();                         // so that no bounded wait spans the previous kernel
-            const uint32_t idesc = t5_idesc_e4m3(256, 256);
-            int st = 0, use = 0, tb = 0, tuse = 0;
-            bool ok = true, ready = false;      // ready: the barriers of this block were seen complete in the last
-            for (long long t = pair; t < tiles && ok; t += pairs)
-                for (int i = 0; i < nb; i++) {
-                    ok = ready || ((tuse == 0 || wait(&tempty[tb], (tuse - 1) & 1, FAULT_GEMV_EMPTY)) &&
-                                   wait(&full[st], use & 1, FAULT_GEMV_FULL));
-                    if (!ok) break;
-                    t5_fence_after();
-                    const uint32_t sa = smem_u32(base + st * MMT_STAGE), sb = sa + FP8_TILE_BYTES, d = tmem + tb * 256;
-                    uint64_t *const e = &empty[st], *const f = &tfull[tb];
-                    if (++st == S) { st = 0; use++; }
-                    if (++tb == 2) { tb = 0; tuse++; }
-                    const bool r0 = tuse == 0 || mbar_test(&tempty[tb], (tuse - 1) & 1);
-                    const bool r1 = mbar_test(&full[st], use & 1);
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        t5_mma2_e4m3(d, t5_desc(sa + 32 * k), t5_desc(sb + 32 * k), idesc, k > 0);
-                    t5_commit2(e);
-                    t5_commit2(f);
-                    ready = r0 && r1;
-                }
+            const uint32_t idesc = t5_idesc_e4m3(256, 256), d = tmem + (warp >> 1) * 256;
+            const uint32_t lo = t5_desc_lo(smem_u32(base));
+            const long long blocks = (tiles - pair + pairs - 1) / pairs * nb - (warp >> 1);
+            int st = warp >> 1, par = 0;
+            bool ready = false;                 // this block's barrier was seen complete in the last round
+            for (long long j = 0; j < blocks; j += 2) {
+                if (!ready && !wait(&full[st], par, FAULT_GEMV_FULL)) break;
+                t5_fence_after();
+                const uint32_t da = lo + st * (MMT_STAGE >> 4), db = da + (FP8_TILE_BYTES >> 4);
+                uint64_t *const f = &done[st];
+                st += 2;
+                par ^= st >= S;
+                st = st >= S ? st - S : st;
+                ready = mbar_test(&full[st], par);
+                t5_mma2_e4m3<false>(d, da, db, idesc);
+                t5_mma2_e4m3<true>(d, da + 2, db + 2, idesc);
+                t5_mma2_e4m3<true>(d, da + 4, db + 4, idesc);
+                t5_mma2_e4m3<true>(d, da + 6, db + 6, idesc);
+                t5_commit2(f);
+            }
             t5_commit2(&drain);
         }
     } else {
-        // ---- sums: lanes 32 * (warp % 4) .. are activation rows, 128 columns one row block ----
+        // ---- sums: lanes 32 * (warp % 4) .. are activation rows, 64 columns lie in one row block ----
         t5_regs_inc<MMT_REGS_SUMS>();
+        const int grp = (warp - 4) >> 2, lrow = rank * 128 + 32 * (warp & 3);
+        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + grp * 64;
+        const uint32_t full0 = t5_cluster_addr(smem_u32(&full[0]), 0);   // rank 0's, 8 bytes each
+        uint8_t *stg = base + S * MMT_STAGE + (warp - 4) * (32 * 64);
+        if (lane == 0) {                                                  // both halves of tensor memory are free
+            t5_cluster_arrive(full0);
+            t5_cluster_arrive(full0 + 8);
+        }
         pdl_wait();
-        const int half = (warp - 4) >> 2, lrow = rank * 128 + 32 * (warp & 3);
-        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 128;
-        uint8_t *stg = base + S * MMT_STAGE + (warp - 4) * (32 * 128);
-        int tb = 0, tuse = 0;
+        int st = 0, par = 0, tb = 0;
         bool ok = true;
         for (long long t = pair; t < tiles && ok; t += pairs) {
             const int m = (int)(t % p.mt), r = (int)(t / p.mt);
             const long long row = (long long)m * 256 + lrow + lane;      // this lane's activation row
-            const int rb = 2 * r + half;
+            const int rb = 2 * r + (grp >> 1);
             const bool live = row < p.a.n && rb < w.rblocks;
             const float *sx = p.a.s + row * p.a.s_ld, *sw = w.scales + (size_t)rb * nb;
-            uint64_t acc[64];
+            uint64_t acc[32];
 #pragma unroll
-            for (int j = 0; j < 64; j++) acc[j] = 0;
-            float x1 = live ? sx[0] : 0.f, w1 = live ? sw[0] : 0.f;
+            for (int j = 0; j < 32; j++) acc[j] = 0;
+            float x1 = live ? *sx : 0.f, w1 = live ? *sw : 0.f;
             for (int i = 0; i < nb; i++) {
                 const float s = x1 * w1;
                 const uint64_t s2 = t5_pair(__float_as_uint(s), __float_as_uint(s));
                 if (live && i + 1 < nb) {                                 // the next block's, while this one is added
-                    x1 = sx[(long long)(i + 1) * p.a.s_inc];
-                    w1 = sw[i + 1];
+                    sx += p.a.s_inc;
+                    sw++;
+                    x1 = *sx;
+                    w1 = *sw;
                 }
-                ok = __all_sync(0xffffffffu, wait(&tfull[tb], tuse & 1, FAULT_GEMV_FULL));
+                ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
                 if (!ok) break;
                 t5_fence_after();
-                uint32_t d[2][32];
-                t5_ld(tcol + tb * 256, d[0]);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    t5_wait_ld(d[c & 1]);
-                    if (c < 3) t5_ld(tcol + tb * 256 + 32 * (c + 1), d[(c + 1) & 1]);
-                    else {
+                    uint32_t d[16];
+                    t5_ld(tcol + tb * 256 + 16 * c, d);
+                    t5_wait_ld(d);
+                    if (c == 3) {
+                        // released for the block after the next, which waits for this on its stage's barrier
                         t5_fence_before();
                         __syncwarp();
-                        if (lane == 0) t5_cluster_arrive(t5_cluster_addr(smem_u32(&tempty[tb]), 0));
+                        if (lane == 0) t5_cluster_arrive(full0 + 8 * (st + 2 >= S ? st + 2 - S : st + 2));
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        acc[c * 16 + j] = t5_fma2(t5_pair(d[c & 1][2 * j], d[c & 1][2 * j + 1]), s2, acc[c * 16 + j]);
+                    for (int j = 0; j < 8; j++)
+                        acc[8 * c + j] = t5_fma2(t5_pair(d[2 * j], d[2 * j + 1]), s2, acc[8 * c + j]);
                 }
-                if (++tb == 2) { tb = 0; tuse++; }
+                st++;
+                par ^= st == S;
+                st = st == S ? 0 : st;
+                tb ^= 1;
             }
             if (!ok || rb >= w.rblocks) continue;
-            // ---- out: 128 bytes of each of the warp's 32 rows at a time, through shared memory ----
-            constexpr int E = 128 / sizeof(TY), V = 16 / sizeof(TY);      // columns a pass, columns a 16-byte chunk
+            // ---- out: 64 bytes of each of the warp's 32 rows at a time, through shared memory ----
+            constexpr int E = 64 / sizeof(TY), V = 16 / sizeof(TY);       // columns a pass, columns a 16-byte chunk
             TY *y = static_cast<TY *>(p.a.y);
 #pragma unroll
-            for (int ps = 0; ps < 128 / E; ps++) {
+            for (int ps = 0; ps < 64 / E; ps++) {
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
+                for (int c = 0; c < 4; c++) {
                     TY v[V];
 #pragma unroll
                     for (int e = 0; e < V; e += 2) {
@@ -481,15 +494,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                         v[e] = fp8_t<TY>(lo);
                         v[e + 1] = fp8_t<TY>(hi);
                     }
-                    *reinterpret_cast<uint4 *>(stg + lane * 128 + ((c ^ (lane & 7)) << 4)) = *reinterpret_cast<uint4 *>(v);
+                    *reinterpret_cast<uint4 *>(stg + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+                        *reinterpret_cast<uint4 *>(v);
                 }
                 __syncwarp();
 #pragma unroll
-                for (int it = 0; it < 8; it++) {
-                    const int lr = it * 4 + (lane >> 3), ch = lane & 7;
+                for (int it = 0; it < 4; it++) {
+                    const int lr = it * 8 + (lane >> 2), ch = lane & 3;
                     const long long orow = (long long)m * 256 + lrow + lr;
-                    const int ocol = rb * FP8_BLOCK + ps * E + ch * V;
-                    const uint4 v = *reinterpret_cast<const uint4 *>(stg + lr * 128 + ((ch ^ (lr & 7)) << 4));
+                    const int ocol = rb * FP8_BLOCK + (grp & 1) * 64 + ps * E + ch * V;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stg + lr * 64 + ((ch ^ ((lr >> 1) & 3)) << 4));
                     if (orow < p.a.n) {
                         TY *o = y + orow * p.a.y_ld + ocol;
                         if (p.vy && ocol + V <= w.rows) {

@@ -15,6 +15,11 @@ __device__ __forceinline__ uint64_t t5_desc(uint32_t saddr) {
            (uint64_t)2 << 61;
 }
 
+// The two words of the same descriptor: the upper does not depend on the
+// address, and 32 bytes further along K is 2 more in the lower.
+#define T5_DESC_HI ((1u << 14) | (2u << 29) | (1024u >> 4))
+__device__ __forceinline__ uint32_t t5_desc_lo(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | 1u << 16; }
+
 // Instruction descriptor of kind::f8f6f4: f32 accumulators, e4m3 operands, both K-major.
 __host__ __device__ constexpr uint32_t t5_idesc_e4m3(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -118,11 +123,13 @@ __device__ __forceinline__ uint32_t t5_cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void t5_mma2_e4m3(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool acc) {
+template <bool ACC>
+__device__ __forceinline__ void t5_mma2_e4m3(uint32_t d, uint32_t da, uint32_t db, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+        "r"(da), "r"(db), "r"(idesc), "n"((int)ACC), "n"(T5_DESC_HI)
         : "memory");
 }
 // As t5_commit, on the barrier at this offset in both CTAs.
