@@ -304,18 +304,17 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
 // that the block will use, `done` (the products' commit, in both CTAs) frees
 // the stage and hands the sums their block.
 //
-// Warps: 0 loads, 1 and 3 products (rank 0), 2 tensor memory, 4-19 sums (four a
-// scheduler: with two, the time that each spends on barriers showed).
-#define MMT_SUM_WARPS 16
+// Warps: 0 loads, 1 and 3 products (rank 0), 2 tensor memory, 4-11 sums.
+#define MMT_SUM_WARPS 8
 #define MMT_THREADS (128 + 32 * MMT_SUM_WARPS)
 #define MMT_STAGES 6
 #define MMT_STAGE (2 * FP8_TILE_BYTES)
 #define MMT_STAGING (MMT_SUM_WARPS * 32 * 64)       // a summing warp's way out: 32 rows x 64 bytes
 #define MMT_SMEM (1024 + MMT_STAGES * MMT_STAGE + MMT_STAGING)
 // Registers a thread at launch, of the first warpgroup and of the summing warps.
-#define MMT_REGS 96
-#define MMT_REGS_FEW 64
-#define MMT_REGS_SUMS 104
+#define MMT_REGS 168
+#define MMT_REGS_FEW 40
+#define MMT_REGS_SUMS 232
 static_assert(128 * MMT_REGS_FEW + 32 * MMT_SUM_WARPS * MMT_REGS_SUMS == MMT_THREADS * MMT_REGS, "register split");
 
 struct Fp8MmtArgs {
@@ -423,67 +422,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             t5_commit2(&drain);
         }
     } else {
-        // ---- sums: lanes 32 * (warp % 4) .. are activation rows, 64 columns lie in one row block ----
+        // ---- sums: lanes 32 * (warp % 4) .. are activation rows, 128 columns one row block ----
         t5_regs_inc<MMT_REGS_SUMS>();
-        const int grp = (warp - 4) >> 2, lrow = rank * 128 + 32 * (warp & 3);
-        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + grp * 64;
+        const int half = (warp - 4) >> 2, lrow = rank * 128 + 32 * (warp & 3);
+        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 128;
         const uint32_t full0 = t5_cluster_addr(smem_u32(&full[0]), 0);   // rank 0's, 8 bytes each
         uint8_t *stg = base + S * MMT_STAGE + (warp - 4) * (32 * 64);
-        if (lane == 0) {                                                  // both halves of tensor memory are free
-            t5_cluster_arrive(full0);
-            t5_cluster_arrive(full0 + 8);
-        }
+        t5_cluster_arrive(full0, lane == 0);                              // both halves of tensor memory are free
+        t5_cluster_arrive(full0 + 8, lane == 0);
         pdl_wait();
         int st = 0, par = 0, tb = 0;
-        bool ok = true;
+        bool ok = true, ready = false;
         for (long long t = pair; t < tiles && ok; t += pairs) {
             const int m = (int)(t % p.mt), r = (int)(t / p.mt);
             const long long row = (long long)m * 256 + lrow + lane;      // this lane's activation row
-            const int rb = 2 * r + (grp >> 1);
-            const bool live = row < p.a.n && rb < w.rblocks;
-            const float *sx = p.a.s + row * p.a.s_ld, *sw = w.scales + (size_t)rb * nb;
-            uint64_t acc[32];
+            const int rb = 2 * r + half;
+            // lanes past the last row and warps past the last block sum what they find and write nothing
+            const float *sx = p.a.s + min(row, (long long)p.a.n - 1) * p.a.s_ld;
+            const float *sw = w.scales + (size_t)min(rb, w.rblocks - 1) * nb;
+            uint64_t acc[64];
 #pragma unroll
-            for (int j = 0; j < 32; j++) acc[j] = 0;
-            float x1 = live ? *sx : 0.f, w1 = live ? *sw : 0.f;
-            for (int i = 0; i < nb; i++) {
-                const float s = x1 * w1;
+            for (int j = 0; j < 64; j++) acc[j] = 0;
+            // Block i; its scales were loaded two blocks ago and their place takes those of block i + 2.
+            auto block = [&](int i, float &x, float &ws) {
+                const float s = x * ws;
                 const uint64_t s2 = t5_pair(__float_as_uint(s), __float_as_uint(s));
-                if (live && i + 1 < nb) {                                 // the next block's, while this one is added
-                    sx += p.a.s_inc;
-                    sw++;
-                    x1 = *sx;
-                    w1 = *sw;
+                const int i2 = min(i + 2, nb - 1);
+                x = sx[i2 * p.a.s_inc];
+                ws = sw[i2];
+                if (!ready && !__all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL))) {
+                    ok = false;
+                    return;
                 }
-                ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
-                if (!ok) break;
                 t5_fence_after();
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t d[16];
-                    t5_ld(tcol + tb * 256 + 16 * c, d);
-                    t5_wait_ld(d);
-                    if (c == 3) {
-                        // released for the block after the next, which waits for this on its stage's barrier
-                        t5_fence_before();
-                        __syncwarp();
-                        if (lane == 0) t5_cluster_arrive(full0 + 8 * (st + 2 >= S ? st + 2 - S : st + 2));
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        acc[8 * c + j] = t5_fma2(t5_pair(d[2 * j], d[2 * j + 1]), s2, acc[8 * c + j]);
-                }
+                // released for the block after the next, which waits for this on its stage's barrier
+                const uint32_t rel = full0 + 8 * (st + 2 >= S ? st + 2 - S : st + 2), src = tcol + tb * 256;
                 st++;
                 par ^= st == S;
                 st = st == S ? 0 : st;
                 tb ^= 1;
+                uint32_t d[2][32];
+                t5_ld(src, d[0]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    t5_wait_ld(d[c & 1]);
+                    if (c < 3) {
+                        t5_ld(src + 32 * (c + 1), d[(c + 1) & 1]);
+                    } else {
+                        t5_fence_before();
+                        t5_cluster_arrive(rel, lane == 0);
+                        ready = __all_sync(0xffffffffu, mbar_test(&done[st], par));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        acc[16 * c + j] = t5_fma2(t5_pair(d[c & 1][2 * j], d[c & 1][2 * j + 1]), s2, acc[16 * c + j]);
+                }
+            };
+            float x0 = sx[0], w0 = sw[0], x1 = sx[min(1, nb - 1) * p.a.s_inc], w1 = sw[min(1, nb - 1)];
+            for (int i = 0; i < nb && ok; i += 2) {
+                block(i, x0, w0);
+                if (ok && i + 1 < nb) block(i + 1, x1, w1);
             }
             if (!ok || rb >= w.rblocks) continue;
             // ---- out: 64 bytes of each of the warp's 32 rows at a time, through shared memory ----
             constexpr int E = 64 / sizeof(TY), V = 16 / sizeof(TY);       // columns a pass, columns a 16-byte chunk
             TY *y = static_cast<TY *>(p.a.y);
 #pragma unroll
-            for (int ps = 0; ps < 64 / E; ps++) {
+            for (int ps = 0; ps < 128 / E; ps++) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     TY v[V];
@@ -502,7 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                 for (int it = 0; it < 4; it++) {
                     const int lr = it * 8 + (lane >> 2), ch = lane & 3;
                     const long long orow = (long long)m * 256 + lrow + lr;
-                    const int ocol = rb * FP8_BLOCK + (grp & 1) * 64 + ps * E + ch * V;
+                    const int ocol = rb * FP8_BLOCK + ps * E + ch * V;
                     const uint4 v = *reinterpret_cast<const uint4 *>(stg + lr * 64 + ((ch ^ ((lr >> 1) & 3)) << 4));
                     if (orow < p.a.n) {
                         TY *o = y + orow * p.a.y_ld + ocol;

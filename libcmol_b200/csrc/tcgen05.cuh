@@ -160,8 +160,11 @@ __device__ __forceinline__ void t5_tma2_2d(void *dst, const CUtensorMap *map, in
 // Arrives on a barrier given by its cluster address.  (Not with a release at
 // cluster scope, which waits for every outstanding access of the thread, ~1000
 // clocks; what the arrival orders here is tensor memory, by the tcgen05 fences.)
-__device__ __forceinline__ void t5_cluster_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void t5_cluster_arrive(uint32_t bar, bool who = true) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar),
+        "r"((uint32_t)who)
+        : "memory");
 }
 
 // Registers of the calling warpgroup, out of those the block was launched with.
