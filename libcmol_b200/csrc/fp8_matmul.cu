@@ -432,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
         t5_cluster_arrive(full0 + 8, lane == 0);
         pdl_wait();
         int st = 0, par = 0, tb = 0;
-        bool ok = true, ready = false;
+        bool ok = true;
         for (long long t = pair; t < tiles && ok; t += pairs) {
             const int m = (int)(t % p.mt), r = (int)(t / p.mt);
             const long long row = (long long)m * 256 + lrow + lane;      // this lane's activation row
@@ -443,35 +443,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             uint64_t acc[64];
 #pragma unroll
             for (int j = 0; j < 64; j++) acc[j] = 0;
-            // Block i; its scales were loaded two blocks ago and their place takes those of block i + 2.
+            uint32_t d[2][32];
+            // Block i, whose first 32 columns are on their way to d[0]; before its last 32 are added, the first
+            // of block i + 1 are sent for.  x and ws, its scales, were loaded two blocks ago and their place
+            // takes those of block i + 2.
             auto block = [&](int i, float &x, float &ws) {
                 const float s = x * ws;
                 const uint64_t s2 = t5_pair(__float_as_uint(s), __float_as_uint(s));
                 const int i2 = min(i + 2, nb - 1);
                 x = sx[i2 * p.a.s_inc];
                 ws = sw[i2];
-                if (!ready && !__all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL))) {
-                    ok = false;
-                    return;
-                }
-                t5_fence_after();
                 // released for the block after the next, which waits for this on its stage's barrier
                 const uint32_t rel = full0 + 8 * (st + 2 >= S ? st + 2 - S : st + 2), src = tcol + tb * 256;
                 st++;
                 par ^= st == S;
                 st = st == S ? 0 : st;
                 tb ^= 1;
-                uint32_t d[2][32];
-                t5_ld(src, d[0]);
+                bool ready = false;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     t5_wait_ld(d[c & 1]);
                     if (c < 3) {
                         t5_ld(src + 32 * (c + 1), d[(c + 1) & 1]);
+                        if (c == 2) ready = __all_sync(0xffffffffu, mbar_test(&done[st], par));
                     } else {
                         t5_fence_before();
                         t5_cluster_arrive(rel, lane == 0);
-                        ready = __all_sync(0xffffffffu, mbar_test(&done[st], par));
+                        if (i + 1 < nb) {
+                            if (!ready) ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
+                            t5_fence_after();
+                            t5_ld(tcol + tb * 256, d[0]);
+                        }
                     }
 #pragma unroll
                     for (int j = 0; j < 16; j++)
@@ -479,10 +481,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                 }
             };
             float x0 = sx[0], w0 = sw[0], x1 = sx[min(1, nb - 1) * p.a.s_inc], w1 = sw[min(1, nb - 1)];
+            ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
+            t5_fence_after();
+            t5_ld(tcol + tb * 256, d[0]);
             for (int i = 0; i < nb && ok; i += 2) {
                 block(i, x0, w0);
                 if (ok && i + 1 < nb) block(i + 1, x1, w1);
             }
+            t5_wait_ld(d[0]);                                             // after a wait that ran out
             if (!ok || rb >= w.rblocks) continue;
             // ---- out: 64 bytes of each of the warp's 32 rows at a time, through shared memory ----
             constexpr int E = 64 / sizeof(TY), V = 16 / sizeof(TY);       // columns a pass, columns a 16-byte chunk

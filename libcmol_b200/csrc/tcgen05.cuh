@@ -157,12 +157,14 @@ __device__ __forceinline__ void t5_tma2_2d(void *dst, const CUtensorMap *map, in
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
-// Arrives on a barrier given by its cluster address.  (Not with a release at
-// cluster scope, which waits for every outstanding access of the thread, ~1000
-// clocks; what the arrival orders here is tensor memory, by the tcgen05 fences.)
-__device__ __forceinline__ void t5_cluster_arrive(uint32_t bar, bool who = true) {
+// Arrives on a barrier given by its cluster address.  Relaxed: what the arrival
+// orders is tensor memory, by the tcgen05 fences around it and the wait for the
+// loads before it; a release at cluster scope waits for every outstanding access
+// of the thread, ~1000 clocks beside loads from global memory.
+__device__ __forceinline__ void t5_cluster_arrive(uint32_t bar, bool who) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar),
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar),
         "r"((uint32_t)who)
         : "memory");
 }
