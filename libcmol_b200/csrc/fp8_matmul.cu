@@ -577,13 +577,11 @@ static bool q_map(CUtensorMap *m, const Fp8MmArgs &a, int rows) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launch with programmatic dependent launch and a (1, cluster, 1) cluster.
+// Launch with programmatic dependent launch and a (1, cluster, 1) cluster; the
+// kernel's attributes are set.
 template <typename P>
 static cudaError_t mm_launch(void (*k)(P), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
                              const P &p) {
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -601,8 +599,8 @@ static cudaError_t mm_launch(void (*k)(P), dim3 grid, int threads, size_t smem, 
     return cudaLaunchKernelEx(&cfg, k, p);
 }
 
-// Largest cluster (16, else the portable 8) in which kernel k runs on the
-// current device.
+// Sets kernel k's attributes on the current device; the largest cluster (16, else
+// the portable 8) in which it runs there, 0 on failure.
 template <typename P>
 static int max_cluster(void (*k)(P), int threads, size_t smem) {
     cudaLaunchConfig_t cfg = {};
@@ -617,10 +615,9 @@ static int max_cluster(void (*k)(P), int threads, size_t smem) {
     cfg.attrs = &at;
     cfg.numAttrs = 1;
     int n = 0;
-    const bool ok =
-        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
-        cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-        cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
+    const bool ok = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0;
     cudaGetLastError();                 // a refused query leaves no error behind
     return ok ? 16 : 8;
 }
@@ -638,7 +635,8 @@ static cudaError_t mmn_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!cluster[dev]) cluster[dev] = max_cluster(k_fp8_mm_n<NT, TY>, MMN_THREADS, Cfg::smem);
+    if (!cluster[dev] && !(cluster[dev] = max_cluster(k_fp8_mm_n<NT, TY>, MMN_THREADS, Cfg::smem)))
+        return cudaErrorInvalidConfiguration;
     const int slots = device_sm_count() * (NT <= 64 ? 2 : 1);
     int ks = (int)std::max<long long>(1, std::min<long long>(std::min<int>(cluster[dev], a.w.kblocks), slots / (tiles * a.w.rblocks)));
     p.kb_per = (a.w.kblocks + ks - 1) / ks;

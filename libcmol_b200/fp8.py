@@ -27,43 +27,71 @@ from . import BF16, F16, F32, CmolError, _vp, check, lib
 BLOCK = 128
 _TAG = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _E4M3 = torch.float8_e4m3fn
+_Q = (_E4M3,)
 
 
 def _blocks(k: int) -> int:
     return (k + BLOCK - 1) // BLOCK
 
 
-def _rows(t, what: str, dtypes, shape, device):
-    """Checks a matrix of consecutive values on `device`; its row stride."""
+def _refuse(t, what: str, dtypes, shape, index: int):
+    """Says what is wrong with a tensor that is not as it should be."""
     if t.dtype not in dtypes:
         raise CmolError(f"{what}: dtype {t.dtype}")
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
-        raise CmolError(f"{what}: shape {tuple(t.shape)}, wanted {shape or 'two dimensions'}")
-    if t.device != device or device.type != "cuda":
-        raise CmolError(f"{what}: on {t.device}, wanted a GPU and one device for all tensors")
-    ld, inc = t.stride()
-    if inc != 1 and t.shape[1] > 1:
-        raise CmolError(f"{what}: the values of a row must be consecutive")
-    return ld
+    if tuple(t.shape) != shape:
+        raise CmolError(f"{what}: shape {tuple(t.shape)}, wanted {shape}")
+    if t.get_device() != index:
+        raise CmolError(f"{what}: on {t.device}, wanted cuda:{index}, as the other tensors")
+    raise CmolError(f"{what}: the values of a row must be consecutive")
 
 
-def _scales(t, what: str, n: int, kb: int, device):
-    if t.dtype != torch.float32 or tuple(t.shape) != (n, kb) or t.device != device:
-        raise CmolError(f"{what}: scales are float32 {(n, kb)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _rows(t, what: str, dtypes, shape, index: int) -> int:
+    """Checks a matrix of consecutive values on GPU `index`; its row stride."""
+    if t.shape == shape and t.dtype in dtypes and t.get_device() == index:
+        ld, inc = t.stride()
+        if inc == 1 or shape[1] == 1:
+            return ld
+    _refuse(t, what, dtypes, shape, index)
+
+
+def _first(t, what: str, dtypes):
+    """As _rows for the tensor that says where and how large: (index, shape, row stride)."""
+    if t.dtype not in dtypes:
+        raise CmolError(f"{what}: dtype {t.dtype}")
+    if t.dim() != 2:
+        raise CmolError(f"{what}: shape {tuple(t.shape)}, wanted two dimensions")
+    index = t.get_device()
+    if index < 0:
+        raise CmolError(f"{what}: on {t.device}, wanted a GPU")
+    shape = tuple(t.shape)
+    return index, shape, _rows(t, what, dtypes, shape, index)
+
+
+def _scales(t, what: str, shape, index: int):
+    if t.shape != shape or t.dtype is not torch.float32 or t.get_device() != index:
+        raise CmolError(f"{what}: scales are float32 {shape} on cuda:{index}, got {t.dtype} {tuple(t.shape)} on "
+                        f"{t.device}")
     return t.stride()
 
 
-def _out(q, scales, what: str, n: int, k: int, device):
+def _out(q, scales, what: str, shape, index: int):
     """The 8-bit output: checked, or new.  New scales keep a block's rows together."""
+    n, k = shape
+    kb = (k + 127) >> 7
     if q is None:
-        q = torch.empty((n, k), dtype=_E4M3, device=device)
+        q = torch.empty(shape, dtype=_E4M3, device=index)
     if scales is None:
-        scales = torch.empty((_blocks(k), n), dtype=torch.float32, device=device).t()
-    return q, _rows(q, what + ": q", (_E4M3,), (n, k), device), scales, _scales(scales, what, n, _blocks(k), device)
+        scales = torch.empty((kb, n), dtype=torch.float32, device=index).t()
+    s_ld, s_inc = _scales(scales, what, (n, kb), index)
+    return q, _rows(q, what, _Q, shape, index), scales, s_ld, s_inc
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The same without building a stream object (2 us a call), where torch offers it.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
 
 
 def rmsnorm(x, norm_w, eps: float = 1e-5, residual=None, residual_out=None, q=None, scales=None):
@@ -73,29 +101,28 @@ def rmsnorm(x, norm_w, eps: float = 1e-5, residual=None, residual_out=None, q=No
     itself when not given); q, scales of norm_w * h / sqrt(mean(h^2) + eps), or
     of h itself when norm_w is None.  x and residual are [n, k] float32,
     float16 or bfloat16, norm_w is [k] float32."""
-    what = "fp8.rmsnorm"
-    dev = x.device
-    x_ld = _rows(x, what + ": x", _TAG, None, dev)
-    n, k = x.shape
-    q, q_ld, scales, (s_ld, s_inc) = _out(q, scales, what, n, k, dev)
+    index, shape, x_ld = _first(x, "fp8.rmsnorm: x", _TAG)
+    n, k = shape
+    q, q_ld, scales, s_ld, s_inc = _out(q, scales, "fp8.rmsnorm: q", shape, index)
     r_ld = ro_ld = r_tag = 0
     r_ptr = ro_ptr = w_ptr = None
     if residual is not None:
-        r_ld = _rows(residual, what + ": residual", _TAG, (n, k), dev)
-        if residual_out is None:
-            residual_out = residual
-        ro_ld = _rows(residual_out, what + ": residual_out", (residual.dtype,), (n, k), dev)
-        r_tag, r_ptr, ro_ptr = _TAG[residual.dtype], residual.data_ptr(), residual_out.data_ptr()
+        r_ld = ro_ld = _rows(residual, "fp8.rmsnorm: residual", _TAG, shape, index)
+        r_tag = _TAG[residual.dtype]
+        r_ptr = ro_ptr = residual.data_ptr()
+        if residual_out is not None and residual_out is not residual:
+            ro_ld = _rows(residual_out, "fp8.rmsnorm: residual_out", (residual.dtype,), shape, index)
+            ro_ptr = residual_out.data_ptr()
     elif residual_out is not None:
-        raise CmolError(f"{what}: residual_out without residual")
+        raise CmolError("fp8.rmsnorm: residual_out without residual")
     if norm_w is not None:
-        if norm_w.dtype != torch.float32 or tuple(norm_w.shape) != (k,) or norm_w.device != dev or (
+        if norm_w.dtype is not torch.float32 or norm_w.shape != (k,) or norm_w.get_device() != index or (
                 k > 1 and norm_w.stride(0) != 1):
-            raise CmolError(f"{what}: norm_w is {k} consecutive float32 values on {dev}")
+            raise CmolError(f"fp8.rmsnorm: norm_w is {k} consecutive float32 values on cuda:{index}")
         w_ptr = norm_w.data_ptr()
-    if lib().cmolcu_fp8_rmsnorm(dev.index, x.data_ptr(), _TAG[x.dtype], x_ld, r_ptr, r_ld, ro_ptr, ro_ld, r_tag, w_ptr,
-                                eps, n, k, q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, _stream(dev)):
-        check(-1, what)
+    if lib().cmolcu_fp8_rmsnorm(index, x.data_ptr(), _TAG[x.dtype], x_ld, r_ptr, r_ld, ro_ptr, ro_ld, r_tag, w_ptr,
+                                eps, n, k, q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, _stream(index)):
+        check(-1, "fp8.rmsnorm")
     return q, scales
 
 
@@ -107,15 +134,13 @@ def quantize(x, q=None, scales=None):
 def swiglu(gate, up, q=None, scales=None):
     """q, scales of gate / (1 + exp(-gate)) * up; gate and up [n, k] of one
     type, which may be halves of one tensor."""
-    what = "fp8.swiglu"
-    dev = gate.device
-    g_ld = _rows(gate, what + ": gate", _TAG, None, dev)
-    n, k = gate.shape
-    u_ld = _rows(up, what + ": up", (gate.dtype,), (n, k), dev)
-    q, q_ld, scales, (s_ld, s_inc) = _out(q, scales, what, n, k, dev)
-    if lib().cmolcu_fp8_swiglu(dev.index, gate.data_ptr(), g_ld, up.data_ptr(), u_ld, _TAG[gate.dtype], n, k,
-                               q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, _stream(dev)):
-        check(-1, what)
+    index, shape, g_ld = _first(gate, "fp8.swiglu: gate", _TAG)
+    u_ld = _rows(up, "fp8.swiglu: up", (gate.dtype,), shape, index)
+    q, q_ld, scales, s_ld, s_inc = _out(q, scales, "fp8.swiglu: q", shape, index)
+    n, k = shape
+    if lib().cmolcu_fp8_swiglu(index, gate.data_ptr(), g_ld, up.data_ptr(), u_ld, _TAG[gate.dtype], n, k,
+                               q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, _stream(index)):
+        check(-1, "fp8.swiglu")
     return q, scales
 
 
@@ -141,31 +166,28 @@ class Fp8Weight:
                             f"on {scales.device}")
         scales = scales.contiguous()
         if q.device.type == "cuda":
-            device = q.device.index
-            ld = _rows(q, what + ": q", (_E4M3,), None, q.device)
+            device, _, ld = _first(q, what + ": q", _Q)
             check(lib().cmolcu_fp8_weight_upload_dev(device, q.data_ptr(), k if rows == 1 else ld,
-                                                     scales.data_ptr(), rows, k, _stream(q.device), C.byref(h)), what)
+                                                     scales.data_ptr(), rows, k, _stream(device), C.byref(h)), what)
         else:
             q = q.contiguous()
             check(lib().cmolcu_fp8_weight_upload(device, q.data_ptr(), scales.data_ptr(), rows, k, C.byref(h)), what)
         self._set(h, rows, k, device)
 
     def _set(self, h, rows, k, device):
-        self.h, self.rows, self.k = h, rows, k
+        self.h, self.rows, self.k, self.index = h, rows, k, device
         self.device = torch.device("cuda", device)
 
     @classmethod
     def quantize(cls, w):
         """A weight from a float32, float16 or bfloat16 [rows, k] matrix on a GPU."""
         what = "Fp8Weight.quantize"
-        ld = _rows(w, what, _TAG, None, w.device)
+        index, (rows, k), ld = _first(w, what, _TAG)
         h = _vp()
-        rows, k = w.shape
-        check(lib().cmolcu_fp8_weight_quantize_dev(w.device.index, w.data_ptr(), _TAG[w.dtype],
-                                                   k if rows == 1 else ld, rows, k, _stream(w.device),
-                                                   C.byref(h)), what)
+        check(lib().cmolcu_fp8_weight_quantize_dev(index, w.data_ptr(), _TAG[w.dtype], k if rows == 1 else ld, rows, k,
+                                                   _stream(index), C.byref(h)), what)
         self = cls.__new__(cls)
-        self._set(h, rows, k, w.device.index)
+        self._set(h, rows, k, index)
         return self
 
     @property
@@ -176,24 +198,23 @@ class Fp8Weight:
         """The weight as it is held: (q [rows, k], scales) on its GPU."""
         q = torch.empty((self.rows, self.k), dtype=_E4M3, device=self.device)
         s = torch.empty((_blocks(self.rows), _blocks(self.k)), dtype=torch.float32, device=self.device)
-        check(lib().cmolcu_fp8_weight_read_dev(self.h, q.data_ptr(), self.k, s.data_ptr(), _stream(self.device)),
+        check(lib().cmolcu_fp8_weight_read_dev(self.h, q.data_ptr(), self.k, s.data_ptr(), _stream(self.index)),
               "Fp8Weight.read")
         return q, s
 
     def matmul(self, q, scales, y=None, dtype=torch.float32):
         """y [n, rows] = (q * scales) . W^T in float32, float16 or bfloat16
         (`y`'s type, else `dtype`)."""
-        what = "Fp8Weight.matmul"
-        dev = self.device
-        q_ld = _rows(q, what + ": q", (_E4M3,), (q.shape[0], self.k), dev)
+        index = self.index
         n = q.shape[0]
-        s_ld, s_inc = _scales(scales, what, n, _blocks(self.k), dev)
+        q_ld = _rows(q, "Fp8Weight.matmul: q", _Q, (n, self.k), index)
+        s_ld, s_inc = _scales(scales, "Fp8Weight.matmul", (n, (self.k + 127) >> 7), index)
         if y is None:
-            y = torch.empty((n, self.rows), dtype=dtype, device=dev)
-        y_ld = _rows(y, what + ": y", _TAG, (n, self.rows), dev)
+            y = torch.empty((n, self.rows), dtype=dtype, device=index)
+        y_ld = _rows(y, "Fp8Weight.matmul: y", _TAG, (n, self.rows), index)
         if lib().cmolcu_fp8_matmul(self.h, q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, n, y.data_ptr(),
-                                   _TAG[y.dtype], y_ld, _stream(dev)):
-            check(-1, what)
+                                   _TAG[y.dtype], y_ld, _stream(index)):
+            check(-1, "Fp8Weight.matmul")
         return y
 
     def free(self):
