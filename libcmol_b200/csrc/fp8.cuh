@@ -5,8 +5,8 @@
 // 2^-126), where amax is the block's largest magnitude: 448 is e4m3's largest
 // value, and the floor keeps 1 / s finite for blocks of zeros or of
 // subnormals.  A NaN in a block makes its scale NaN, an infinity makes the
-// scale infinite (and its own q NaN): either way every product with the block
-// is NaN or infinite, as it is without the rounding to 8 bits.
+// scale infinite, and the q of such a block are NaN: every product with it is
+// NaN, as it is NaN or infinite without the rounding to 8 bits.
 #pragma once
 #include "common.cuh"
 
@@ -64,32 +64,52 @@ __device__ __forceinline__ __half fp8_t<__half>(float v) { return __float2half_r
 template <>
 __device__ __forceinline__ __nv_bfloat16 fp8_t<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive elements as they lie in memory: 16-byte accesses where
-// `vec` says that the address is 16-byte aligned, single elements otherwise.
-template <typename T>
-struct Fp8Oct {
-    T e[8];
-    __device__ __forceinline__ void load(const T *p, bool vec) {
-        if (vec) {
+// V consecutive elements as they lie in memory, in accesses of 32 or 16 bytes
+// (`vec` 2 or 1: the address is a multiple of that) or one by one (0).
+template <typename T, int V>
+struct Fp8Vec {
+    static constexpr int B = V * (int)sizeof(T);
+    static_assert(B % 16 == 0, "whole 16-byte accesses");
+    alignas(32) T e[V];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(e) / 16; i++)
+        for (int i = 0; i < B / 16; i++) reinterpret_cast<uint4 *>(e)[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T *p, int vec) {
+        if (B % 32 == 0 && vec == 2) {
+            uint32_t *r = reinterpret_cast<uint32_t *>(e);
+#pragma unroll
+            for (int i = 0; i < B / 32; i++)
+                asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(r[8 * i]), "=r"(r[8 * i + 1]), "=r"(r[8 * i + 2]), "=r"(r[8 * i + 3]),
+                               "=r"(r[8 * i + 4]), "=r"(r[8 * i + 5]), "=r"(r[8 * i + 6]), "=r"(r[8 * i + 7])
+                             : "l"(reinterpret_cast<const uint8_t *>(p) + 32 * i));
+        } else if (vec) {
+#pragma unroll
+            for (int i = 0; i < B / 16; i++)
                 reinterpret_cast<uint4 *>(e)[i] = *(reinterpret_cast<const uint4 *>(p) + i);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) e[i] = p[i];
+            for (int i = 0; i < V; i++) e[i] = p[i];
         }
     }
-    __device__ __forceinline__ void store(T *p, bool vec) const {
+    __device__ __forceinline__ void store(T *p, int vec) const {
         if (vec) {
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(e) / 16; i++)
+            for (int i = 0; i < B / 16; i++)
                 *(reinterpret_cast<uint4 *>(p) + i) = reinterpret_cast<const uint4 *>(e)[i];
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = e[i];
+            for (int i = 0; i < V; i++) p[i] = e[i];
         }
     }
 };
+
+// The widest access that every row of a buffer starts on.
+inline int fp8_vec(const void *p, long long ld_bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)ld_bytes;
+    return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
+}
 
 // max(a, |b|) that keeps a NaN of either side.
 __device__ __forceinline__ float fp8_amax(float a, float b) {
@@ -98,10 +118,18 @@ __device__ __forceinline__ float fp8_amax(float a, float b) {
     return r;
 }
 
-// Scale of a block from its largest magnitude.
+// Scale of a block from its largest magnitude: within 2^-23 of amax / 448.
 __device__ __forceinline__ float fp8_scale(float amax) {
-    const float s = __fdiv_rn(amax, 448.f), lo = 1.17549435e-38f;
+    const float s = amax * (1.f / 448.f), lo = 1.17549435e-38f;
     return s < lo ? lo : s;           // a NaN passes
+}
+
+// 1 / s of a scale (2^-126 <= s <= 2^120, or infinite or NaN, which give NaN):
+// the approximate reciprocal and one Newton step, within 2^-24.
+__device__ __forceinline__ float fp8_inv(float s) {
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return fmaf(r, fmaf(-s, r, 1.f), r);
 }
 
 // Two e4m3 values, the first in the low byte (round to nearest even; a NaN
@@ -117,12 +145,24 @@ __device__ __forceinline__ uint2 fp8_pack8(const float v[8], float inv) {
                       fp8_pack2(v[4] * inv, v[5] * inv) | fp8_pack2(v[6] * inv, v[7] * inv) << 16);
 }
 
-// Largest magnitude of the 128 values that 16 consecutive lanes hold, 8 each.
-__device__ __forceinline__ float fp8_amax16(const float v[8]) {
+// V e4m3 values to consecutive bytes (V-byte aligned).
+template <int V>
+__device__ __forceinline__ void fp8_store(uint8_t *q, const float v[V], float inv) {
+    if constexpr (V == 8) {
+        *reinterpret_cast<uint2 *>(q) = fp8_pack8(v, inv);
+    } else {
+        const uint2 a = fp8_pack8(v, inv), b = fp8_pack8(v + 8, inv);
+        *reinterpret_cast<uint4 *>(q) = make_uint4(a.x, a.y, b.x, b.y);
+    }
+}
+
+// Largest magnitude of the 128 values that 128 / V consecutive lanes hold, V each.
+template <int V>
+__device__ __forceinline__ float fp8_block_amax(const float v[V]) {
     float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) a = fp8_amax(a, v[i]);
+    for (int i = 0; i < V; i++) a = fp8_amax(a, v[i]);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = fp8_amax(a, __shfl_xor_sync(0xffffffffu, a, o));
+    for (int o = FP8_BLOCK / V / 2; o > 0; o >>= 1) a = fp8_amax(a, __shfl_xor_sync(0xffffffffu, a, o));
     return a;
 }

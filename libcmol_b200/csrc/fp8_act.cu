@@ -15,6 +15,35 @@ struct Fp8Out {
     long long s_ld, s_inc;
 };
 
+// Values a lane holds of a row: 32 bytes of x, so that the work a lane does once
+// (addresses, a block's scale) is shared by 16 values of the 16-bit types.
+template <typename T>
+constexpr int lane_values() { return 32 / (int)sizeof(T); }
+
+struct Fp8None {};
+
+struct Fp8ActArgs {
+    const void *x, *r;        // input; residual (norm, quantise) or second input (SwiGLU)
+    void       *r_out;
+    long long   x_ld, r_ld, r_out_ld;
+    const float *g;           // norm gains
+    float       eps;
+    int         n, k;
+    int         vx, vr, vo, vg;   // access widths of x, r, r_out, g (fp8_vec)
+    Fp8Out      o;
+};
+
+// Writes V values of (row, chunk c) in 8 bits; the lanes of a block call it
+// together, those past the row with zeros and `in` false.
+template <int V>
+__device__ __forceinline__ void put(const Fp8Out &o, long long row, int c, const float v[V], bool in) {
+    const float s = fp8_scale(fp8_block_amax<V>(v));
+    if (!in) return;
+    fp8_store<V>(o.q + row * o.q_ld + (long long)c * V, v, fp8_inv(s));
+    constexpr int L = FP8_BLOCK / V;
+    if (c % L == 0) o.s[row * o.s_ld + (long long)(c / L) * o.s_inc] = s;
+}
+
 // ---------------------------------------------------------------------------
 // RMS norm
 // ---------------------------------------------------------------------------
@@ -24,177 +53,211 @@ struct Fp8Out {
 //
 // Bound by memory: x and r are read once and stay in registers between the
 // sum of squares and the output.  A row is held by W warps (blockDim.x =
-// 32 W), 8 consecutive values a lane and C such octets; the 128 values of a
-// block are 16 lanes of one warp, so its amax is four shuffles.  Rows longer
-// than a CTA holds (k > 65536) are read twice.
-struct Fp8NormArgs {
-    const void  *x, *r;
-    void        *r_out;
-    long long    x_ld, r_ld, r_out_ld;
-    const float *g;           // NULL: no norm
-    float        eps;
-    int          n, k;
-    int          vx, vr, vo, vg;   // 16-byte accesses of x, r, r_out, g
-    Fp8Out       o;
+// 32 W), V consecutive values a lane and C such chunks; the 128 values of a
+// block are 8 or 16 lanes of one warp, so its amax is three or four shuffles.  A
+// CTA goes through its rows with the next row's loads on their way and the gains
+// in registers.  Rows longer than 12 warps hold (k > 12288) are read twice.
+template <typename TX, typename TR, int C>
+struct NormRow {
+    static constexpr int  V = lane_values<TX>();
+    static constexpr bool RES = !std::is_same<TR, Fp8None>::value;
+    using TRV = typename std::conditional<RES, TR, TX>::type;
+    Fp8Vec<TX, V>  x[C];
+    Fp8Vec<TRV, V> r[RES ? C : 1];
+    // chunks base + i * T + t of a row
+    __device__ __forceinline__ void load(const Fp8ActArgs &a, long long row, int first, int T) {
+        const int nchunk = a.k / V;
+        const TX *xr = static_cast<const TX *>(a.x) + row * a.x_ld;
+        const TRV *rr = static_cast<const TRV *>(a.r) + row * a.r_ld;
+#pragma unroll
+        for (int i = 0; i < C; i++) {
+            const int c = first + i * T;
+            x[i].zero();
+            if (c < nchunk) x[i].load(xr + (long long)c * V, a.vx);
+            if constexpr (RES) {
+                r[i].zero();
+                if (c < nchunk) r[i].load(rr + (long long)c * V, a.vr);
+            }
+        }
+    }
+    __device__ __forceinline__ void sum(float (&v)[C][V]) const {
+#pragma unroll
+        for (int i = 0; i < C; i++)
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                v[i][e] = fp8_f(x[i].e[e]);
+                if constexpr (RES) v[i][e] += fp8_f(r[i].e[e]);
+            }
+    }
+    __device__ __forceinline__ static void store_sum(const Fp8ActArgs &a, long long row, int c, const float (&v)[V]) {
+        if constexpr (RES) {
+            Fp8Vec<TRV, V> h;
+#pragma unroll
+            for (int e = 0; e < V; e++) h.e[e] = fp8_t<TRV>(v[e]);
+            h.store(static_cast<TRV *>(a.r_out) + row * a.r_out_ld + (long long)c * V, a.vo);
+        }
+    }
 };
 
-struct Fp8None {};
+// Sum over the T threads of a row; red: a float a warp, of this row's own.
+__device__ __forceinline__ float row_sum(float v, int T, float *red) {
+    v = warp_sum(v);
+    if (T > 32) {                                          // blockDim.y is 1 when a row has several warps
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) red[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = warp_sum(lane < (T >> 5) ? red[lane] : 0.f);
+    }
+    return v;
+}
 
-// Most warps a row: octets of 8 f32 values in registers bound the threads.
-static constexpr int norm_warps(int c) { return c == 1 ? 32 : c == 8 ? 8 : 16; }
+#define NORM_WARPS 12         // most warps a row
 
 template <typename TX, typename TR, int C>
-__global__ void __launch_bounds__(32 * norm_warps(C)) k_fp8_norm(const Fp8NormArgs a) {
-    constexpr bool RES = !std::is_same<TR, Fp8None>::value;
+__global__ void __launch_bounds__(32 * NORM_WARPS) k_fp8_norm(const Fp8ActArgs a) {
+    using Row = NormRow<TX, TR, C>;
+    constexpr int V = Row::V;
+    const int T = blockDim.x, t = threadIdx.x, nchunk = a.k / V;
+    const long long step = (long long)gridDim.x * blockDim.y;
+    long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    __shared__ float red[2][NORM_WARPS];
+    int flip = 0;
     pdl_wait();
     pdl_launch_dependents();
-    const int T = blockDim.x, t = threadIdx.x, lane = t & 31;
-    const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-    const bool live = row < a.n;
-    const int nchunk = a.k >> 3;
-    const int iters = (nchunk - 1) / (T * C) + 1;
-    float v[C][8];
-
-    auto load = [&](int it) {
-        Fp8Oct<TX> x[C];
-        const TX *xr = static_cast<const TX *>(a.x) + row * a.x_ld;
+    Row x;
+    if (row < a.n) x.load(a, row, t, T);
+    Fp8Vec<float, V> g[C];
 #pragma unroll
-        for (int i = 0; i < C; i++) {
-            const int c = (it * C + i) * T + t;
-            if (live && c < nchunk) x[i].load(xr + (long long)c * 8, a.vx);
-        }
-        if constexpr (RES) {
-            Fp8Oct<TR> r[C];
-            const TR *rr = static_cast<const TR *>(a.r) + row * a.r_ld;
-#pragma unroll
-            for (int i = 0; i < C; i++) {
-                const int c = (it * C + i) * T + t;
-                if (live && c < nchunk) r[i].load(rr + (long long)c * 8, a.vr);
-            }
-#pragma unroll
-            for (int i = 0; i < C; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    v[i][e] = live && (it * C + i) * T + t < nchunk ? fp8_f(x[i].e[e]) + fp8_f(r[i].e[e]) : 0.f;
-        } else {
-#pragma unroll
-            for (int i = 0; i < C; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    v[i][e] = live && (it * C + i) * T + t < nchunk ? fp8_f(x[i].e[e]) : 0.f;
-        }
-    };
-
-    float ir = 1.f;
-    if (a.g) {
-        float ss = 0.f;
-        for (int it = 0; it < iters; it++) {
-            load(it);
-#pragma unroll
-            for (int i = 0; i < C; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) ss = __fmaf_rn(v[i][e], v[i][e], ss);
-        }
-        ss = warp_sum(ss);
-        if (T > 32) {
-            __shared__ float red[32];                  // blockDim.y is 1 when a row has several warps
-            if (lane == 0) red[t >> 5] = ss;
-            __syncthreads();
-            ss = warp_sum(lane < (T >> 5) ? red[lane] : 0.f);
-        }
-        ir = 1.0f / sqrtf(ss / (float)a.k + a.eps);
+    for (int i = 0; i < C; i++) {
+        g[i].zero();
+        if (i * T + t < nchunk) g[i].load(a.g + (long long)(i * T + t) * V, a.vg);
     }
-    for (int it = 0; it < iters; it++) {
-        if (!a.g || iters > 1) load(it);
+    for (; row < a.n; row += step) {                        // the rows of a CTA with several warps a row: all or none
+        float v[C][V], ss = 0.f;
+        x.sum(v);
+        if (row + step < a.n) x.load(a, row + step, t, T);
+#pragma unroll
+        for (int i = 0; i < C; i++)
+#pragma unroll
+            for (int e = 0; e < V; e++) ss = __fmaf_rn(v[i][e], v[i][e], ss);
+        ss = row_sum(ss, T, red[flip]);
+        flip ^= 1;
+        const float ir = 1.0f / sqrtf(ss / (float)a.k + a.eps);
 #pragma unroll
         for (int i = 0; i < C; i++) {
-            const int c = (it * C + i) * T + t;
-            const bool in = live && c < nchunk;
-            if constexpr (RES) {
-                if (in) {
-                    Fp8Oct<TR> h;
+            const int c = i * T + t;
+            const bool in = c < nchunk;
+            if (in) Row::store_sum(a, row, c, v[i]);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) h.e[e] = fp8_t<TR>(v[i][e]);
-                    h.store(static_cast<TR *>(a.r_out) + row * a.r_out_ld + (long long)c * 8, a.vo);
-                }
-            }
-            if (a.g) {
-                Fp8Oct<float> g;
-                if (in) g.load(a.g + (long long)c * 8, a.vg);
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[i][e] = in ? g.e[e] * (v[i][e] * ir) : 0.f;
-            }
-            const float s = fp8_scale(fp8_amax16(v[i]));
-            if (in) {
-                *reinterpret_cast<uint2 *>(a.o.q + row * a.o.q_ld + (long long)c * 8) =
-                    fp8_pack8(v[i], __frcp_rn(s));
-                if ((lane & 15) == 0) a.o.s[row * a.o.s_ld + (long long)(c >> 4) * a.o.s_inc] = s;
-            }
+            for (int e = 0; e < V; e++) v[i][e] = g[i].e[e] * (v[i][e] * ir);
+            put<V>(a.o, row, c, v[i], in);
         }
+    }
+}
+
+// Rows longer than a CTA's registers hold: one CTA a row, read twice.
+template <typename TX, typename TR>
+__global__ void __launch_bounds__(512) k_fp8_norm_long(const Fp8ActArgs a) {
+    using Row = NormRow<TX, TR, 1>;
+    constexpr int V = Row::V;
+    const int T = blockDim.x, t = threadIdx.x, nchunk = a.k / V;
+    const long long row = blockIdx.x;
+    __shared__ float red[16];
+    pdl_wait();
+    pdl_launch_dependents();
+    Row x;
+    float v[1][V], ss = 0.f;
+    for (int c = t; c < nchunk; c += T) {
+        x.load(a, row, c, T);
+        x.sum(v);
+#pragma unroll
+        for (int e = 0; e < V; e++) ss = __fmaf_rn(v[0][e], v[0][e], ss);
+    }
+    const float ir = 1.0f / sqrtf(row_sum(ss, T, red) / (float)a.k + a.eps);
+    for (int c0 = 0; c0 < nchunk; c0 += T) {                // whole warps: the lanes of a block stay together
+        const int c = c0 + t;
+        const bool in = c < nchunk;
+        Fp8Vec<float, V> g;
+        g.zero();
+        if (in) g.load(a.g + (long long)c * V, a.vg);
+        x.load(a, row, c, T);
+        x.sum(v);
+        if (in) Row::store_sum(a, row, c, v[0]);
+#pragma unroll
+        for (int e = 0; e < V; e++) v[0][e] = g.e[e] * (v[0][e] * ir);
+        put<V>(a.o, row, c, v[0], in);
     }
 }
 
 template <typename TX, typename TR>
-static cudaError_t norm_launch(const Fp8NormArgs &a, cudaStream_t st) {
-    const int chunks = (a.k + 255) / 256;              // warps a row at one octet a lane
-    int c = 8;
-    while (c > 1 && (long long)a.n * ((chunks + c - 1) / c) < 148 * 16) c >>= 1;
-    while (c < 8 && (chunks + c - 1) / c > norm_warps(c)) c <<= 1;
-    const int w = std::min(norm_warps(c), (chunks + c - 1) / c);
-    const int rows = w == 1 ? 4 : 1;
-    const dim3 grid((unsigned)((a.n - 1) / rows + 1)), block(32 * w, rows);
-    switch (c) {
-    case 1: return launch_k(k_fp8_norm<TX, TR, 1>, grid, block, 0, st, true, a);
-    case 2: return launch_k(k_fp8_norm<TX, TR, 2>, grid, block, 0, st, true, a);
-    case 4: return launch_k(k_fp8_norm<TX, TR, 4>, grid, block, 0, st, true, a);
-    default: return launch_k(k_fp8_norm<TX, TR, 8>, grid, block, 0, st, true, a);
-    }
+static cudaError_t norm_launch(const Fp8ActArgs &a, cudaStream_t st) {
+    constexpr int V = lane_values<TX>(), CMAX = 32 / V;     // at most 32 values of a row a lane
+    const int sms = device_sm_count(), warps = (a.k / V + 31) / 32;
+    if (warps > NORM_WARPS * CMAX)
+        return launch_k(k_fp8_norm_long<TX, TR>, dim3((unsigned)a.n), dim3(512), 0, st, true, a);
+    // One chunk a lane where that leaves SMs with little to do; more where there are rows enough: fewer warps wait
+    // for one another and for the row's sum.
+    int c = 1;
+    while (c < CMAX && ((warps + c - 1) / c > NORM_WARPS || (long long)a.n * ((warps + c - 1) / c) > sms * 16LL)) c <<= 1;
+    const int w = (warps + c - 1) / c, rows = w == 1 ? 4 : 1;
+    const long long ctas = ((long long)a.n - 1) / rows + 1;
+    const int per_sm = std::max(1, 16 / (w * rows));        // resident warps that keep memory busy
+    const dim3 grid((unsigned)std::min<long long>(ctas, (long long)sms * per_sm)), block(32 * w, rows);
+    if (c == 1) return launch_k(k_fp8_norm<TX, TR, 1>, grid, block, 0, st, true, a);
+    if (c == 2) return launch_k(k_fp8_norm<TX, TR, 2>, grid, block, 0, st, true, a);
+    if constexpr (CMAX >= 4) return launch_k(k_fp8_norm<TX, TR, 4>, grid, block, 0, st, true, a);
+    return cudaErrorInvalidValue;
 }
 
 // ---------------------------------------------------------------------------
-// SwiGLU
+// Value by value: SwiGLU, and the 8-bit form of x (+ r) as it is
 // ---------------------------------------------------------------------------
-//   v = gate / (1 + exp(-gate)) * up,  (q, s) of v
-struct Fp8SwigluArgs {
-    const void *g, *u;
-    long long   g_ld, u_ld;
-    int         n, k;
-    int         vg, vu;
-    Fp8Out      o;
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) k_fp8_swiglu(const Fp8SwigluArgs a) {
+//   SwiGLU: v = x / (1 + exp(-x)) * r;  else h = x + r, r' = rn(h), v = h
+// A thread takes one chunk of a row.  exp and the quotient are the fast forms
+// (each within a few 2^-24 here, against the 2^-4 of the output).  Bound by memory
+// for f32, by instructions for the 16-bit types.
+template <typename TX, typename TR, bool SWIGLU>
+__global__ void __launch_bounds__(256) k_fp8_map(const Fp8ActArgs a) {
+    using Row = NormRow<TX, TR, 1>;
+    constexpr int V = Row::V;
     pdl_wait();
     pdl_launch_dependents();
-    const long long row = blockIdx.x;
-    const int c = blockIdx.y * 256 + threadIdx.x;
-    const bool in = c < (a.k >> 3);
-    Fp8Oct<T> g, u;
-    if (in) {
-        g.load(static_cast<const T *>(a.g) + row * a.g_ld + (long long)c * 8, a.vg);
-        u.load(static_cast<const T *>(a.u) + row * a.u_ld + (long long)c * 8, a.vu);
-    }
-    float v[8];
+    const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    const int c = blockIdx.y * blockDim.x + threadIdx.x;
+    const bool in = row < a.n && c < a.k / V;
+    float v[1][V];
+    Row x;
+    if (in) x.load(a, row, c, 0);
+    if constexpr (SWIGLU) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float x = fp8_f(g.e[e]);
-        v[e] = in ? x / (1.0f + expf(-x)) * fp8_f(u.e[e]) : 0.f;
+        for (int e = 0; e < V; e++) {
+            const float g = fp8_f(x.x[0].e[e]);
+            v[0][e] = in ? __fdividef(g, 1.0f + __expf(-g)) * fp8_f(x.r[0].e[e]) : 0.f;
+        }
+    } else {
+        x.sum(v);
+        if (in) Row::store_sum(a, row, c, v[0]);
+#pragma unroll
+        for (int e = 0; e < V; e++) v[0][e] = in ? v[0][e] : 0.f;
     }
-    const float s = fp8_scale(fp8_amax16(v));
-    if (in) {
-        *reinterpret_cast<uint2 *>(a.o.q + row * a.o.q_ld + (long long)c * 8) = fp8_pack8(v, __frcp_rn(s));
-        if ((threadIdx.x & 15) == 0) a.o.s[row * a.o.s_ld + (long long)(c >> 4) * a.o.s_inc] = s;
-    }
+    put<V>(a.o, row, c, v[0], in);
+}
+
+template <typename TX, typename TR, bool SWIGLU>
+static cudaError_t map_launch(const Fp8ActArgs &a, cudaStream_t st) {
+    constexpr int V = lane_values<TX>(), L = FP8_BLOCK / V;
+    const int chunks = a.k / V, span = (chunks + L - 1) / L * L;      // whole blocks
+    // a narrow row takes part of a CTA (whole warps in all), a wide one several
+    const int bx = span <= 64 ? span : std::min(256, (span + 31) / 32 * 32);
+    const int by = bx <= 64 ? 256 / bx / 4 * 4 : std::max(1, 256 / bx);
+    const dim3 grid((unsigned)((a.n - 1) / by + 1), (unsigned)((chunks - 1) / bx + 1)), block(bx, by);
+    if (grid.y > 65535) return cudaErrorInvalidConfiguration;
+    return launch_k(k_fp8_map<TX, TR, SWIGLU>, grid, block, 0, st, true, a);
 }
 
 // ---------------------------------------------------------------------------
 // C ABI
 // ---------------------------------------------------------------------------
-static bool aligned16(const void *p, long long ld, int elem) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem) % 16 == 0;
-}
-
 // Checks of the 8-bit output; 0 or -1 with the message set.
 static int out_check(const char *who, int n, int k, void *q, long long q_ld, const float *s, long long s_ld,
                      long long s_inc) {
@@ -236,20 +299,24 @@ extern "C" int cmolcu_fp8_rmsnorm(int device, const void *x, int x_dtype, long l
     }
     Fp8Device dev(device);
     CUDA_TRY(dev.err);
-    Fp8NormArgs a = {};
+    Fp8ActArgs a = {};
     a.x = x; a.x_ld = x_ld;
     a.r = res; a.r_ld = res_ld;
     a.r_out = res_out; a.r_out_ld = res_out_ld;
     a.g = norm_w; a.eps = eps; a.n = n; a.k = k;
-    a.vx = aligned16(x, n > 1 ? x_ld : 0, xb);
-    a.vr = aligned16(res, n > 1 ? res_ld : 0, rb);
-    a.vo = aligned16(res_out, n > 1 ? res_out_ld : 0, rb);
-    a.vg = aligned16(norm_w, 0, 4);
+    a.vx = fp8_vec(x, n > 1 ? x_ld * xb : 0);
+    a.vr = fp8_vec(res, n > 1 ? res_ld * rb : 0);
+    a.vo = fp8_vec(res_out, n > 1 ? res_out_ld * rb : 0);
+    a.vg = fp8_vec(norm_w, 0);
     a.o = {static_cast<uint8_t *>(q), q_ld, scales, s_ld, s_inc};
+    const cudaStream_t st = (cudaStream_t)stream;
     CUDA_TRY(fp8_with_type(x_dtype, [&](auto tx) {
         using TX = decltype(tx);
-        if (!res) return norm_launch<TX, Fp8None>(a, (cudaStream_t)stream);
-        return fp8_with_type(res_dtype, [&](auto tr) { return norm_launch<TX, decltype(tr)>(a, (cudaStream_t)stream); });
+        if (!res) return norm_w ? norm_launch<TX, Fp8None>(a, st) : map_launch<TX, Fp8None, false>(a, st);
+        return fp8_with_type(res_dtype, [&](auto tr) {
+            using TR = decltype(tr);
+            return norm_w ? norm_launch<TX, TR>(a, st) : map_launch<TX, TR, false>(a, st);
+        });
     }));
     return 0;
 }
@@ -265,15 +332,13 @@ extern "C" int cmolcu_fp8_swiglu(int device, const void *gate, long long gate_ld
     if (!gate || !up) { cmolcu_set_error("%s: NULL argument", who); return -1; }
     Fp8Device dev(device);
     CUDA_TRY(dev.err);
-    Fp8SwigluArgs a = {};
-    a.g = gate; a.g_ld = gate_ld; a.u = up; a.u_ld = up_ld; a.n = n; a.k = k;
-    a.vg = aligned16(gate, n > 1 ? gate_ld : 0, eb);
-    a.vu = aligned16(up, n > 1 ? up_ld : 0, eb);
+    Fp8ActArgs a = {};
+    a.x = gate; a.x_ld = gate_ld; a.r = up; a.r_ld = up_ld; a.n = n; a.k = k;
+    a.vx = fp8_vec(gate, n > 1 ? gate_ld * eb : 0);
+    a.vr = fp8_vec(up, n > 1 ? up_ld * eb : 0);
     a.o = {static_cast<uint8_t *>(q), q_ld, scales, s_ld, s_inc};
-    const dim3 grid((unsigned)n, (unsigned)((k - 1) / 2048 + 1));
-    if (grid.y > 65535) { cmolcu_set_error("%s: k=%d is too long", who, k); return -1; }
     CUDA_TRY(fp8_with_type(dtype, [&](auto t) {
-        return launch_k(k_fp8_swiglu<decltype(t)>, grid, dim3(256), 0, (cudaStream_t)stream, true, a);
+        return map_launch<decltype(t), decltype(t), true>(a, (cudaStream_t)stream);
     }));
     return 0;
 }

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) k_fp8_weight_quant(const T *src, long lon
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const long long row = (long long)rb * FP8_BLOCK + i * 16 + (tid >> 4);
-        Fp8Oct<T> o;
+        Fp8Vec<T, 8> o;
         const bool in = row < w.rows && col < w.k;
         if (in) o.load(src + row * ld + col, vec);
 #pragma unroll
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) k_fp8_weight_quant(const T *src, long lon
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; i++) amax = fp8_amax(amax, red[i]);
-    const float s = fp8_scale(amax), inv = __frcp_rn(s);
+    const float s = fp8_scale(amax), inv = fp8_inv(s);
     uint8_t *t = tiles + ((size_t)rb * w.kblocks + kb) * FP8_TILE_BYTES;
 #pragma unroll
     for (int i = 0; i < 8; i++)
@@ -171,7 +171,7 @@ extern "C" int cmolcu_fp8_weight_quantize_dev(int device, const void *w, int dty
     CUDA_TRY(dev.err);
     cmolcu_fp8_weight_t *h = nullptr;
     if (weight_new(who, device, rows, k, &h)) return -1;
-    const int vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (ld * eb) % 16 == 0;
+    const int vec = fp8_vec(w, ld * eb);
     const cudaError_t e = fp8_with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return launch_k(k_fp8_weight_quant<T>, dim3(h->w.kblocks, h->w.rblocks), dim3(256), 0, (cudaStream_t)stream,

@@ -85,7 +85,7 @@ STEP = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
 
 # every width of the kernel's choice of lanes, ragged last blocks, a row that is read twice
 @pytest.mark.parametrize("n, k", [(1, 16), (1, 960), (3, 576), (5, 128), (2, 144), (257, 2048), (33, 8192), (700, 11008),
-                                  (2, 16400), (1, 40016), (1500, 256), (4099, 64)])
+                                  (2, 12288), (2, 16400), (1, 40016), (1500, 256), (4099, 64), (9000, 960), (3, 3824)])
 @pytest.mark.parametrize("xt, rt", [(F32, F32), (BF16, BF16), (F16, None), (BF16, F32)])
 def test_rmsnorm(n, k, xt, rt):
     from libcmol_b200 import fp8
@@ -101,7 +101,7 @@ def test_rmsnorm(n, k, xt, rt):
         assert ((out.double() - h).abs() <= (STEP[rt] + U) * h.abs() + 2 ** -25).all()
 
 
-@pytest.mark.parametrize("n, k", [(1, 16), (7, 960), (300, 2064), (9, 17008)])
+@pytest.mark.parametrize("n, k", [(1, 16), (7, 960), (300, 2064), (9, 17008), (130, 400), (77, 64), (3, 992)])
 @pytest.mark.parametrize("xt", [F32, F16, BF16])
 def test_quantize(n, k, xt):
     from libcmol_b200 import fp8
@@ -181,7 +181,7 @@ def test_broadcast_row():
     _check_eight_bits(_norm_ref(x.expand(6, 576), r, w, 1e-5)[1], q, s, _norm_delta(576))
 
 
-@pytest.mark.parametrize("n, k", [(1, 16), (1, 2560), (6, 144), (301, 8192), (64, 11008), (3, 2064), (1000, 48)])
+@pytest.mark.parametrize("n, k", [(1, 16), (1, 2560), (6, 144), (301, 8192), (64, 11008), (3, 2064), (1000, 48), (130, 400), (5, 208)])
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 def test_swiglu(n, k, t):
     from libcmol_b200 import fp8
