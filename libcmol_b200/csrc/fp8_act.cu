@@ -111,16 +111,17 @@ __device__ __forceinline__ float row_sum(float v, int T, float *red) {
     return v;
 }
 
-#define NORM_WARPS 12         // most warps a row
+// Most warps a row: the chunks a lane holds bound the threads that the registers allow.
+static constexpr int norm_warps(int c) { return c == 1 ? 24 : c == 2 ? 16 : 12; }
 
 template <typename TX, typename TR, int C>
-__global__ void __launch_bounds__(32 * NORM_WARPS) k_fp8_norm(const Fp8ActArgs a) {
+__global__ void __launch_bounds__(32 * norm_warps(C)) k_fp8_norm(const Fp8ActArgs a) {
     using Row = NormRow<TX, TR, C>;
     constexpr int V = Row::V;
     const int T = blockDim.x, t = threadIdx.x, nchunk = a.k / V;
     const long long step = (long long)gridDim.x * blockDim.y;
     long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-    __shared__ float red[2][NORM_WARPS];
+    __shared__ float red[2][norm_warps(C)];
     int flip = 0;
     pdl_wait();
     pdl_launch_dependents();
@@ -193,16 +194,20 @@ template <typename TX, typename TR>
 static cudaError_t norm_launch(const Fp8ActArgs &a, cudaStream_t st) {
     constexpr int V = lane_values<TX>(), CMAX = 32 / V;     // at most 32 values of a row a lane
     const int sms = device_sm_count(), warps = (a.k / V + 31) / 32;
-    if (warps > NORM_WARPS * CMAX)
+    if (warps > norm_warps(CMAX) * CMAX)
         return launch_k(k_fp8_norm_long<TX, TR>, dim3((unsigned)a.n), dim3(512), 0, st, true, a);
-    // One chunk a lane where that leaves SMs with little to do; more where there are rows enough: fewer warps wait
-    // for one another and for the row's sum.
-    int c = 1;
-    while (c < CMAX && ((warps + c - 1) / c > NORM_WARPS || (long long)a.n * ((warps + c - 1) / c) > sms * 16LL)) c <<= 1;
+    // Chunks a lane and resident warps an SM, as measured (us, 1 / 2 chunks): a few rows are latency, spread over
+    // all lanes (1x960 f32 1.6 / 1.9); up to a wave, fewer warps that wait for the row's sum (256x2048 f32 3.2 / 2.7,
+    // 1000x960 bf16 3.3 / 3.1); many rows of up to 8 warps want warps (8191x2048 bf16 20.5 / 21.2, 8192x960 f32 17.8 /
+    // 17.9), longer ones fewer at the barrier (2048x8192 bf16 24.2 / 22.2).
+    const long long rw = (long long)a.n * warps;
+    int c = rw <= sms * 4LL || (rw > sms * 32LL && warps <= 8) ? 1 : 2;
+    const int resident = c == 1 ? 48 : 32;
+    while (c < CMAX && (warps + c - 1) / c > norm_warps(c)) c <<= 1;
     const int w = (warps + c - 1) / c, rows = w == 1 ? 4 : 1;
     const long long ctas = ((long long)a.n - 1) / rows + 1;
-    const int per_sm = std::max(1, 16 / (w * rows));        // resident warps that keep memory busy
-    const dim3 grid((unsigned)std::min<long long>(ctas, (long long)sms * per_sm)), block(32 * w, rows);
+    const dim3 grid((unsigned)std::min<long long>(ctas, (long long)sms * std::max(1, resident / (w * rows))));
+    const dim3 block(32 * w, rows);
     if (c == 1) return launch_k(k_fp8_norm<TX, TR, 1>, grid, block, 0, st, true, a);
     if (c == 2) return launch_k(k_fp8_norm<TX, TR, 2>, grid, block, 0, st, true, a);
     if constexpr (CMAX >= 4) return launch_k(k_fp8_norm<TX, TR, 4>, grid, block, 0, st, true, a);
