@@ -283,39 +283,45 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
 // Many rows of activations: they are the tensor core's M
 // ---------------------------------------------------------------------------
 // Two CTAs (a cluster on neighbouring SMs) form one tile of 256 activation rows
-// x 256 weight rows: each holds 128 of both in shared memory, and every product
-// of the pair (M = N = 256) reads both halves, so an SM loads 32 KB a block of
-// 128 along k for work that takes its tensor core 512 clocks.  A lane of
-// tensor memory is an activation row here and a warp's 128 columns are one
-// row block of the weight, so a block's scale is one number a thread: taking a
-// block's product from tensor memory and adding it (128 columns a thread, two
-// values an instruction) measured ~300 clocks an SM, which hides behind the
-// products, as the double buffer in tensor memory lets both run at once.
-// (With the roles of the operands as in k_fp8_mm_n the scale differs from column
-// to column and comes from shared memory: 670 clocks.)
+// x N weight rows: each holds half of both in shared memory, and every product
+// of the pair (M = 256) reads both halves, so at N = 256 an SM loads 32 KB a block
+// of 128 along k for work that takes its tensor core 512 clocks.  A lane of
+// tensor memory is an activation row here, so a block's scale is one number a
+// thread for every 128 columns: taking a block's product from tensor memory and
+// adding it (128 columns a thread, two values an instruction) measured ~300
+// clocks an SM alone, which hides behind the products.  (With the roles of the
+// operands as in k_fp8_mm_n the scale differs from column to column and comes
+// from shared memory: 670 clocks.)
 //
 // The CTAs are persistent: loads and products run on into the next tile while
-// the sums of the last are written.
+// the sums of the last are written.  N is chosen so that the tiles fill the
+// pairs of SMs evenly (mmt_launch).
 //
 // A wait or an arrival costs a thread about as much as two products cost it to
-// issue, so two warps issue in turn (the two halves of tensor memory), and there
-// are two barriers a block: `full` counts the bytes of both
-// CTAs' stages and the 32 summing warps' release of the half of tensor memory
-// that the block will use, `done` (the products' commit, in both CTAs) frees
-// the stage and hands the sums their block.
+// issue, so two warps issue in turn, and there are two barriers a block: `full`
+// counts the bytes of both CTAs' stages and the 16 summing warps' release of the
+// part of tensor memory that the block will use, `done` (the products' commit,
+// in both CTAs) frees the stage and hands the sums their block.
 //
 // Warps: 0 loads, 1 and 3 products (rank 0), 2 tensor memory, 4-11 sums.
 #define MMT_SUM_WARPS 8
 #define MMT_THREADS (128 + 32 * MMT_SUM_WARPS)
-#define MMT_STAGES 6
-#define MMT_STAGE (2 * FP8_TILE_BYTES)
-#define MMT_STAGING (MMT_SUM_WARPS * 32 * 64)       // a summing warp's way out: 32 rows x 64 bytes
-#define MMT_SMEM (1024 + MMT_STAGES * MMT_STAGE + MMT_STAGING)
 // Registers a thread at launch, of the first warpgroup and of the summing warps.
 #define MMT_REGS 168
 #define MMT_REGS_FEW 40
 #define MMT_REGS_SUMS 232
 static_assert(128 * MMT_REGS_FEW + 32 * MMT_SUM_WARPS * MMT_REGS_SUMS == MMT_THREADS * MMT_REGS, "register split");
+
+template <int N>
+struct MmtCfg {
+    static constexpr int rows = N / 2;                                      // weight rows of a CTA, columns of a sum
+    static constexpr int bufs = 512 / N;                                    // products in tensor memory
+    static constexpr int stage = FP8_TILE_BYTES + rows * FP8_BLOCK;
+    static constexpr int staging = MMT_SUM_WARPS * 32 * 64;                 // a summing warp's way out: 32 rows x 64 bytes
+    static constexpr int stages = (226 * 1024 - 1024 - staging) / stage / 2 * 2;
+    static constexpr int smem = 1024 + stages * stage + staging;
+    static_assert(N == 128 || N == 256, "a CTA's rows lie in one row block");
+};
 
 struct Fp8MmtArgs {
     CUtensorMap tm_q, tm_w;    // activations as above; weight tiles as rows of 128 bytes
@@ -325,10 +331,11 @@ struct Fp8MmtArgs {
     unsigned   *fault;
 };
 
-template <typename TY>
+template <int N, typename TY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp8_mm_t(const __grid_constant__ Fp8MmtArgs p) {
-    constexpr int S = MMT_STAGES;
-    static_assert(S % 2 == 0 && S >= 4, "a stage belongs to one half of tensor memory");
+    using Cfg = MmtCfg<N>;
+    constexpr int S = Cfg::stages, B = Cfg::bufs, R = Cfg::rows, CH = 32, NC = R / CH;
+    static_assert(S % 2 == 0, "a stage belongs to one of the two issuing warps");
     const Fp8W &w = p.a.w;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)t5_cluster_rank();
@@ -377,17 +384,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             bool ok = true;
             for (long long t = pair; t < tiles && ok; t += pairs) {
                 const int m = (int)(t % p.mt), r = (int)(t / p.mt);
-                const int row = m * 256 + rank * 128, rb = 2 * r + rank;
+                const int row = m * 256 + rank * 128, wrow = r * N + rank * R;
                 for (int i = 0; i < nb; i++) {
                     if (use > 0 && !wait(&done[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) {
                         ok = false;
                         break;
                     }
-                    uint8_t *dst = base + st * MMT_STAGE;
-                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * MMT_STAGE);
+                    uint8_t *dst = base + st * Cfg::stage;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * Cfg::stage);
                     const uint32_t bar = t5_cluster_addr(smem_u32(&full[st]), 0);
                     t5_tma2_2d(dst, &p.tm_q, i * FP8_BLOCK, row, bar);
-                    t5_tma2_2d(dst + FP8_TILE_BYTES, &p.tm_w, 0, (rb * nb + i) * FP8_BLOCK, bar);
+                    t5_tma2_2d(dst + FP8_TILE_BYTES, &p.tm_w, 0, ((wrow >> 7) * nb + i) * FP8_BLOCK + (wrow & 127), bar);
                     if (++st == S) { st = 0; use++; }
                 }
             }
@@ -399,19 +406,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
         } else if ((warp & 1) && lane == 0 && rank == 0) {
             // ---- products: warp 1 the even blocks, warp 3 the odd ones ----
             pdl_wait();                         // so that no bounded wait spans the previous kernel
-            const uint32_t idesc = t5_idesc_e4m3(256, 256), d = tmem + (warp >> 1) * 256;
+            const uint32_t idesc = t5_idesc_e4m3(256, N);
             const uint32_t lo = t5_desc_lo(smem_u32(base));
-            const long long blocks = (tiles - pair + pairs - 1) / pairs * nb - (warp >> 1);
-            int st = warp >> 1, par = 0;
+            const long long blocks = (tiles - pair + pairs - 1) / pairs * nb;
+            int st = warp >> 1, par = 0, buf = warp >> 1;
             bool ready = false;                 // this block's barrier was seen complete in the last round
-            for (long long j = 0; j < blocks; j += 2) {
+            for (long long j = warp >> 1; j < blocks; j += 2) {
                 if (!ready && !wait(&full[st], par, FAULT_GEMV_FULL)) break;
                 t5_fence_after();
-                const uint32_t da = lo + st * (MMT_STAGE >> 4), db = da + (FP8_TILE_BYTES >> 4);
+                const uint32_t da = lo + st * (Cfg::stage >> 4), db = da + (FP8_TILE_BYTES >> 4);
+                const uint32_t d = tmem + buf * N;
                 uint64_t *const f = &done[st];
                 st += 2;
                 par ^= st >= S;
                 st = st >= S ? st - S : st;
+                buf = buf + 2 >= B ? buf + 2 - B : buf + 2;
                 ready = mbar_test(&full[st], par);
                 t5_mma2_e4m3<false>(d, da, db, idesc);
                 t5_mma2_e4m3<true>(d, da + 2, db + 2, idesc);
@@ -422,82 +431,84 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             t5_commit2(&drain);
         }
     } else {
-        // ---- sums: lanes 32 * (warp % 4) .. are activation rows, 128 columns one row block ----
+        // ---- sums: lanes 32 * (warp % 4) .. are activation rows, R columns of a warp weight rows ----
         t5_regs_inc<MMT_REGS_SUMS>();
         const int half = (warp - 4) >> 2, lrow = rank * 128 + 32 * (warp & 3);
-        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 128;
+        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * R;
         const uint32_t full0 = t5_cluster_addr(smem_u32(&full[0]), 0);   // rank 0's, 8 bytes each
-        uint8_t *stg = base + S * MMT_STAGE + (warp - 4) * (32 * 64);
-        t5_cluster_arrive(full0, lane == 0);                              // both halves of tensor memory are free
-        t5_cluster_arrive(full0 + 8, lane == 0);
+        uint8_t *stg = base + S * Cfg::stage + (warp - 4) * (32 * 64);
+#pragma unroll
+        for (int i = 0; i < B; i++) t5_cluster_arrive(full0 + 8 * i, lane == 0);   // tensor memory is free
         pdl_wait();
-        int st = 0, par = 0, tb = 0;
+        int st = 0, par = 0, buf = 0;
         bool ok = true;
         for (long long t = pair; t < tiles && ok; t += pairs) {
             const int m = (int)(t % p.mt), r = (int)(t / p.mt);
             const long long row = (long long)m * 256 + lrow + lane;      // this lane's activation row
-            const int rb = 2 * r + half;
+            const int wrow = r * N + half * R, rb = wrow >> 7;            // this warp's first weight row, its block
             // lanes past the last row and warps past the last block sum what they find and write nothing
             const float *sx = p.a.s + min(row, (long long)p.a.n - 1) * p.a.s_ld;
             const float *sw = w.scales + (size_t)min(rb, w.rblocks - 1) * nb;
-            uint64_t acc[64];
+            uint64_t acc[R / 2];
 #pragma unroll
-            for (int j = 0; j < 64; j++) acc[j] = 0;
-            uint32_t d[2][32];
-            // Block i, whose first 32 columns are on their way to d[0]; before its last 32 are added, the first
-            // of block i + 1 are sent for.  x and ws, its scales, were loaded two blocks ago and their place
-            // takes those of block i + 2.
+            for (int j = 0; j < R / 2; j++) acc[j] = 0;
+            uint32_t d[2][CH];
+            // Block i, whose first 32 columns are on their way to d[0]; before its last 32 are added, the first of
+            // block i + 1 are sent for.  x and ws, its scales, were loaded two blocks ago and their place takes those
+            // of block i + 2.
             auto block = [&](int i, float &x, float &ws) {
                 const float s = x * ws;
                 const uint64_t s2 = t5_pair(__float_as_uint(s), __float_as_uint(s));
                 const int i2 = min(i + 2, nb - 1);
                 x = sx[i2 * p.a.s_inc];
                 ws = sw[i2];
-                // released for the block after the next, which waits for this on its stage's barrier
-                const uint32_t rel = full0 + 8 * (st + 2 >= S ? st + 2 - S : st + 2), src = tcol + tb * 256;
+                // released for the block B blocks on, which waits for this on its stage's barrier
+                const uint32_t rel = full0 + 8 * (st + B >= S ? st + B - S : st + B), src = tcol + buf * N;
                 st++;
                 par ^= st == S;
                 st = st == S ? 0 : st;
-                tb ^= 1;
+                buf = buf + 1 == B ? 0 : buf + 1;
                 bool ready = false;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    t5_wait_ld(d[c & 1]);
-                    if (c < 3) {
-                        t5_ld(src + 32 * (c + 1), d[(c + 1) & 1]);
-                        if (c == 2) ready = __all_sync(0xffffffffu, mbar_test(&done[st], par));
+                for (int c = 0; c < NC; c++) {
+                    uint32_t(&dc)[CH] = d[c & 1], (&dn)[CH] = d[(c + 1) & 1];
+                    t5_wait_ld(dc);
+                    if (c < NC - 1) {
+                        t5_ld(src + CH * (c + 1), dn);
+                        if (c == NC - 2) ready = __all_sync(0xffffffffu, mbar_test(&done[st], par));
                     } else {
                         t5_fence_before();
                         t5_cluster_arrive(rel, lane == 0);
                         if (i + 1 < nb) {
                             if (!ready) ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
                             t5_fence_after();
-                            t5_ld(tcol + tb * 256, d[0]);
+                            t5_ld(tcol + buf * N, dn);
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        acc[16 * c + j] = t5_fma2(t5_pair(d[c & 1][2 * j], d[c & 1][2 * j + 1]), s2, acc[16 * c + j]);
+                    for (int j = 0; j < CH / 2; j++)
+                        acc[CH / 2 * c + j] = t5_fma2(t5_pair(dc[2 * j], dc[2 * j + 1]), s2, acc[CH / 2 * c + j]);
                 }
             };
-            float x0 = sx[0], w0 = sw[0], x1 = sx[min(1, nb - 1) * p.a.s_inc], w1 = sw[min(1, nb - 1)];
+            const int i1 = min(1, nb - 1);
+            float x0 = sx[0], w0 = sw[0], x1 = sx[i1 * p.a.s_inc], w1 = sw[i1];
             ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
             t5_fence_after();
-            t5_ld(tcol + tb * 256, d[0]);
+            t5_ld(tcol + buf * N, d[0]);
             for (int i = 0; i < nb && ok; i += 2) {
                 block(i, x0, w0);
                 if (ok && i + 1 < nb) block(i + 1, x1, w1);
             }
-            t5_wait_ld(d[0]);                                             // after a wait that ran out
             if (!ok || rb >= w.rblocks) continue;
             // ---- out: 64 bytes of each of the warp's 32 rows at a time, through shared memory ----
-            constexpr int E = 64 / sizeof(TY), V = 16 / sizeof(TY);       // columns a pass, columns a 16-byte chunk
+            constexpr int E = 64 / (int)sizeof(TY), V = 16 / (int)sizeof(TY);   // columns a pass, a 16-byte chunk
+            auto place = [&](int lr, int c) { return stg + lr * 64 + ((c ^ ((lr >> 1) & 3)) << 4); };
             TY *y = static_cast<TY *>(p.a.y);
 #pragma unroll
-            for (int ps = 0; ps < 128 / E; ps++) {
+            for (int ps = 0; ps < R / E; ps++) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    TY v[V];
+                    alignas(16) TY v[V];
 #pragma unroll
                     for (int e = 0; e < V; e += 2) {
                         float lo, hi;
@@ -505,16 +516,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                         v[e] = fp8_t<TY>(lo);
                         v[e + 1] = fp8_t<TY>(hi);
                     }
-                    *reinterpret_cast<uint4 *>(stg + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-                        *reinterpret_cast<uint4 *>(v);
+                    *reinterpret_cast<uint4 *>(place(lane, c)) = *reinterpret_cast<uint4 *>(v);
                 }
                 __syncwarp();
 #pragma unroll
                 for (int it = 0; it < 4; it++) {
                     const int lr = it * 8 + (lane >> 2), ch = lane & 3;
                     const long long orow = (long long)m * 256 + lrow + lr;
-                    const int ocol = rb * FP8_BLOCK + ps * E + ch * V;
-                    const uint4 v = *reinterpret_cast<const uint4 *>(stg + lr * 64 + ((ch ^ ((lr >> 1) & 3)) << 4));
+                    const int ocol = wrow + ps * E + ch * V;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(place(lr, ch));
                     if (orow < p.a.n) {
                         TY *o = y + orow * p.a.y_ld + ocol;
                         if (p.vy && ocol + V <= w.rows) {
@@ -645,28 +655,29 @@ static cudaError_t mmn_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     return mm_launch(k_fp8_mm_n<NT, TY>, grid, MMN_THREADS, Cfg::smem, p.ksplit, st, p);
 }
 
-// Weight tiles as rows of 128 bytes, read a tile at a time (their bytes are in
+// Weight tiles as rows of 128 bytes, read `rows` at a time (their bytes are in
 // the operand's swizzled order already); row blocks past the last read as zero.
-static bool w_map(CUtensorMap *m, const Fp8W &w) {
+static bool w_map(CUtensorMap *m, const Fp8W &w, int rows) {
     const encode_t enc = encode_fn();
     if (!enc) return false;
     const cuuint64_t dims[2] = {FP8_BLOCK, (cuuint64_t)w.rblocks * w.kblocks * FP8_BLOCK};
     const cuuint64_t strides[1] = {FP8_BLOCK};
-    const cuuint32_t box[2] = {FP8_BLOCK, FP8_BLOCK}, es[2] = {1u, 1u};
+    const cuuint32_t box[2] = {FP8_BLOCK, (cuuint32_t)rows}, es[2] = {1u, 1u};
     return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(w.tiles), dims, strides, box, es,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename TY>
+template <int N, typename TY>
 static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
-    const auto kern = k_fp8_mm_t<TY>;
+    using Cfg = MmtCfg<N>;
+    const auto kern = k_fp8_mm_t<N, TY>;
     Fp8MmtArgs p = {};
     p.a = a;
     p.fault = fault;
-    if (!q_map(&p.tm_q, a, FP8_BLOCK) || !w_map(&p.tm_w, a.w)) return cudaErrorInvalidValue;
+    if (!q_map(&p.tm_q, a, FP8_BLOCK) || !w_map(&p.tm_w, a.w, Cfg::rows)) return cudaErrorInvalidValue;
     p.mt = (a.n - 1) / 256 + 1;
-    p.rt = (a.w.rblocks - 1) / 2 + 1;
+    p.rt = (a.w.rows - 1) / N + 1;
     p.vy = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.n == 1 || (a.y_ld * sizeof(TY)) % 16 == 0);
     // the register split of the kernel adds up only to what it was built with
     static std::atomic<int> ready[64];
@@ -677,13 +688,25 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
         cudaFuncAttributes fa = {};
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);
         if (e == cudaSuccess && fa.numRegs != MMT_REGS) e = cudaErrorInvalidConfiguration;
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MMT_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem);
         if (e != cudaSuccess) return e;
         ready[dev] = 1;
     }
     const long long tiles = (long long)p.mt * p.rt;
     const int pairs = (int)std::min<long long>(tiles, device_sm_count() / 2);
-    return launch_k(kern, dim3(2 * pairs), dim3(MMT_THREADS), MMT_SMEM, st, true, p);
+    return launch_k(kern, dim3(2 * pairs), dim3(MMT_THREADS), Cfg::smem, st, true, p);
+}
+
+// Weight rows of a pair's tile.  A round of 128-row tiles over the pairs of SMs
+// takes 0.62 to 0.72 of one of 256-row tiles (0.33 against 0.47 us a block of 128
+// along k): the narrow ones win where they leave fewer pairs idle (777x2049x8192
+// 32.3 / 47.9 us, 256x22016x2048 20.7 / 22.8, 1000x2048x2048 9.5 / 12.1), the wide
+// ones elsewhere (8192x22016x2048 429 / 370).
+template <typename TY>
+static cudaError_t mmt_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
+    const long long mt = (a.n - 1) / 256 + 1, pairs = std::max(1, device_sm_count() / 2);
+    auto rounds = [&](int n) { return (mt * ((a.w.rows - 1) / n + 1) + pairs - 1) / pairs; };
+    return rounds(128) * 62 < rounds(256) * 100 ? mmt_launch<128, TY>(a, fault, st) : mmt_launch<256, TY>(a, fault, st);
 }
 
 extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld, const float *scales,
@@ -716,7 +739,7 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
         if (n <= 32) return mmn_launch<32, TY>(a, fault, st);
         if (n <= 64) return mmn_launch<64, TY>(a, fault, st);
         if (n <= 128) return mmn_launch<128, TY>(a, fault, st);
-        return mmt_launch<TY>(a, fault, st);
+        return mmt_pick<TY>(a, fault, st);
     }));
     return 0;
 }
