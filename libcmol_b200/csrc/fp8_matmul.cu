@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 struct Fp8MmArgs {
     Fp8W           w;
@@ -24,6 +25,111 @@ struct Fp8MmArgs {
     void          *y;
     long long      y_ld;
 };
+
+// ---------------------------------------------------------------------------
+// Up to 16 rows of activations: straight from memory
+// ---------------------------------------------------------------------------
+// Bound by the weights' stream, so what counts is that it divides evenly over the
+// SMs and that nothing stands between a load and its use: no ring, no tensor
+// memory, no cluster.  A warp takes 16 weight rows and every KW-th block of 128
+// along k; what it loads (16 bytes a lane and row) is, as it lies in registers,
+// the operand of the warp-wide product m16n8k32: the order of k within a block is
+// the same permutation for both operands.  A block's product starts from zero and
+// is scaled and added in f32.  The KW warps of the same rows add up through shared
+// memory, in order.  (tcgen05 takes 128 rows at once, from shared memory: a ring,
+// 172 CTAs for 22016 rows on 148 SMs and a cluster's sum where rows are few; it
+// measured 11.3 us at 1x22016x2048 and 13.2 us at 1x2048x11008.)
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int few_warps(int kw) { return kw > 8 ? kw : 8; }
+
+template <int NG, int KW, typename TY>
+__global__ void __launch_bounds__(32 * few_warps(KW), KW > 8 ? 1 : 2) k_fp8_mm_few(const Fp8MmArgs a) {
+    constexpr int D = 2, W = few_warps(KW), RG = W / KW;                  // blocks in flight; warps, row groups of a CTA
+    const Fp8W &w = a.w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kw = warp % KW, rg = warp / KW;
+    const int g = lane >> 2, t = lane & 3;                                // row (column for b) and quarter of a fragment
+    const int r0 = (blockIdx.x * RG + rg) * 16;                           // rows [r0, r0 + 16)
+    const int nb = r0 < w.rows ? w.kblocks : 0;
+    const uint8_t *wt = w.tiles + (size_t)(r0 >> 7) * nb * FP8_TILE_BYTES + ((r0 & 127) + g) * 128;
+    const float *sw = w.scales + (size_t)(r0 >> 7) * nb;
+    const int o0 = (t ^ g) << 4, o1 = ((t + 4) ^ g) << 4;                 // 16-byte chunks t and t + 4 of rows g, g + 8
+    uint4 wr[D][4], x[D][NG][2];
+    float s[D][NG][2], ws[D];
+    auto load_w = [&](int d, int b) {
+        if (b >= nb) return;
+        const uint8_t *p = wt + (size_t)b * FP8_TILE_BYTES;
+        wr[d][0] = ld_stream_u4(p + o0);
+        wr[d][1] = ld_stream_u4(p + 1024 + o0);
+        wr[d][2] = ld_stream_u4(p + o1);
+        wr[d][3] = ld_stream_u4(p + 1024 + o1);
+        ws[d] = sw[b];
+    };
+    auto load_x = [&](int d, int b) {
+        if (b >= nb) return;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            const int c = 8 * j + g;
+            const uint8_t *xp = a.q + c * a.q_ld + (long long)b * FP8_BLOCK + 16 * t;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                x[d][j][h] = make_uint4(0, 0, 0, 0);
+                if (c < a.n && b * FP8_BLOCK + 64 * h + 16 * t < w.k) x[d][j][h] = *reinterpret_cast<const uint4 *>(xp + 64 * h);
+                const int cc = 8 * j + 2 * t + h;                         // the column of accumulators h and 2 + h
+                s[d][j][h] = a.s[min(cc, a.n - 1) * a.s_ld + b * a.s_inc];   // past the last column: not written
+            }
+        }
+    };
+    float acc[NG][4];
+#pragma unroll
+    for (int j = 0; j < NG; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll
+    for (int d = 0; d < D; d++) load_w(d, kw + d * KW);                   // weights do not wait for the previous kernel
+    pdl_wait();
+    pdl_launch_dependents();
+#pragma unroll
+    for (int d = 0; d < D; d++) load_x(d, kw + d * KW);
+    for (int b0 = kw; b0 < nb; b0 += D * KW) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            if (b0 + d * KW >= nb) break;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                float v[2][4] = {};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint4 &p = wr[d][2 * h], &q = wr[d][2 * h + 1], &b = x[d][j][h];
+                    mma_e4m3(v[h], p.x, q.x, p.y, q.y, b.x, b.y);
+                    mma_e4m3(v[h], p.z, q.z, p.w, q.w, b.z, b.w);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[j][i] = __fmaf_rn(v[0][i] + v[1][i], s[d][j][i & 1] * ws[d], acc[j][i]);
+            }
+            load_w(d, b0 + (D + d) * KW);
+            load_x(d, b0 + (D + d) * KW);
+        }
+    }
+    __shared__ float part[W][8 * NG][16];
+#pragma unroll
+    for (int j = 0; j < NG; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) part[warp][8 * j + 2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[j][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < RG * 128 * NG; i += 32 * W) {    // (row group, column, row)
+        const int r = i & 15, c = (i >> 4) % (8 * NG), gg = i / (128 * NG), row = (blockIdx.x * RG + gg) * 16 + r;
+        float y = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; k++) y += part[gg * KW + k][c][r];
+        if (row < w.rows && c < a.n) static_cast<TY *>(a.y)[c * a.y_ld + row] = fp8_t<TY>(y);
+    }
+}
 
 // ---------------------------------------------------------------------------
 // Few rows of activations: the weights' rows are the tensor core's M
@@ -38,38 +144,53 @@ struct Fp8MmArgs {
 // Bound by the weights' stream (one byte a value, read once per NT activation
 // rows): 16 KB blocks, contiguous along k, come by bulk copies into a ring.
 // Where the row blocks are fewer than the SMs, k is split over the CTAs of a
-// cluster, which add their sums through distributed shared memory in the
-// order of the split.
+// cluster.  Each owns some of the columns: the others store their sums into its
+// ring, once its last product has read it (stores to another CTA are not waited
+// for; loading them took longer than the rest of the sum), and after a barrier it
+// adds them in the order of the split.
 //
-// Warps: 0 weights' producer, 1 tensor memory and products, 2 activations'
-// producer, 3 scales, 4-11 sums.
+// Barriers, two a block as in k_fp8_mm_t: `full` counts both operands' bytes and
+// the summing warps' release of tensor memory, `done` is the product's commit.
+// Scales come eight blocks at a time.
+//
+// Warps: 0 loads, 1 and 2 products in turn (1 also tensor memory), 3 scales, 4-11
+// sums.
 #define MMN_THREADS 384
 #define MMN_SUM_WARPS 8
-#define MMN_SCALE_SLOTS 8
-#define MMN_MAX_STAGES 8
+#define MMN_GROUP 8            // blocks whose scales come together
+#define MMN_MAX_SPLIT 8        // CTAs of a cluster (16 measured slower: 16x2048x11008 15.6 us against 8.5)
 
 struct Fp8MmnArgs {
     CUtensorMap tm_q;          // activations: [n][k] bytes, box 128 x NT, 128-byte swizzle
     Fp8MmArgs   a;
     int         ksplit;        // CTAs of a cluster
     int         kb_per;        // k blocks of a CTA
+    int         own;           // columns of a CTA of a cluster (the last may have fewer)
     unsigned   *fault;
 };
 
 template <int NT>
 struct MmnCfg {
-    static constexpr int bufs = NT >= 128 ? 2 : 4;                        // products in tensor memory
-    static constexpr int cols = bufs * NT < 32 ? 32 : bufs * NT;
+    static constexpr int per_sm = NT <= 64 ? 2 : 1;
+    // Registers a thread where 32 columns' sums need more than two CTAs an SM leave (0: no split), of the first
+    // warpgroup and of the summing warps.
+    static constexpr int regs = NT == 64 ? 80 : 0, regs_few = 40, regs_sums = 96;
+    static_assert(128 * regs_few + 256 * regs_sums <= 384 * 80, "register split");
     static constexpr int stage = FP8_TILE_BYTES + NT * FP8_BLOCK;
-    static constexpr int stages = (100 * 1024) / stage < MMN_MAX_STAGES ? (100 * 1024) / stage : MMN_MAX_STAGES;
-    static constexpr int smem = 1024 + stages * stage + MMN_SCALE_SLOTS * NT * 4;
-    static_assert(stages * stage >= NT * FP8_BLOCK * 4, "the sums of a CTA fit in its ring");
+    static constexpr int scales = 2 * MMN_GROUP * NT * 4;
+    static constexpr int stages = ((per_sm == 2 ? 110 : 190) * 1024 - 1024 - scales) / stage / 2 * 2;
+    static constexpr int bufs = NT <= 64 ? 4 : 2;                         // products in tensor memory
+    static constexpr int cols = bufs * NT < 32 ? 32 : bufs * NT;
+    static constexpr int smem = 1024 + stages * stage + scales;
+    static_assert((NT + MMN_MAX_SPLIT) * FP8_BLOCK * 4 <= stages * stage, "ksplit * own columns fit in the ring");
+    static_assert(stages >= bufs, "a buffer's release counts on a later block's stage");
 };
 
 template <int NT, typename TY>
-__global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(const __grid_constant__ Fp8MmnArgs p) {
+__global__ void __launch_bounds__(MMN_THREADS, MmnCfg<NT>::per_sm) k_fp8_mm_n(const __grid_constant__ Fp8MmnArgs p) {
     using Cfg = MmnCfg<NT>;
     constexpr int S = Cfg::stages, B = Cfg::bufs, C = NT / 2;             // C: columns of a summing warp
+    constexpr int CH = C < 16 || NT > 64 ? (C < 32 ? C : 32) : 16, NC = C / CH, G = MMN_GROUP;
     const Fp8W &w = p.a.w;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long c0 = (long long)blockIdx.x * NT;                      // first activation row
@@ -78,8 +199,9 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
     const int cols = (int)min((long long)NT, p.a.n - c0);
 
     uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)cmolcu_smem + 1023) & ~(uintptr_t)1023);
-    float *scales = reinterpret_cast<float *>(base + S * Cfg::stage);     // [slot][NT]
-    __shared__ uint64_t full[S], empty[S], tfull[B], tempty[B], sfull[MMN_SCALE_SLOTS], sempty[MMN_SCALE_SLOTS], drain;
+    float *scales = reinterpret_cast<float *>(base + S * Cfg::stage);     // [2 * G blocks][NT]
+    float *part = reinterpret_cast<float *>(base);                        // [ksplit][own][128], over the drained ring
+    __shared__ uint64_t full[S], done[S], sfull[2], sempty[2], drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;                                               // a bounded wait ran out: every role gives up
     volatile int *aborted = &s_abort;
@@ -87,18 +209,14 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
     if (tid == 0) {
         t5_prefetch_map(&p.tm_q);
         for (int i = 0; i < S; i++) {
-            mbar_init(&full[i], 2);                                       // both producers, with their bytes
-            mbar_init(&empty[i], 1);
+            mbar_init(&full[i], 1 + MMN_SUM_WARPS);
+            mbar_init(&done[i], 1);
         }
-        for (int i = 0; i < B; i++) {
-            mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], MMN_SUM_WARPS);
-        }
-        for (int i = 0; i < MMN_SCALE_SLOTS; i++) {
+        for (int i = 0; i < 2; i++) {
             mbar_init(&sfull[i], 1);
             mbar_init(&sempty[i], MMN_SUM_WARPS);
         }
-        mbar_init(&drain, 1);
+        mbar_init(&drain, 2);
         fence_mbar_init();
         s_abort = 0;
     }
@@ -117,125 +235,167 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
         return false;
     };
 
-    uint64_t acc[C / 2];                                                  // sums of this lane's row, two columns each
-#pragma unroll
-    for (int i = 0; i < C / 2; i++) acc[i] = 0;
-
-    if (warp == 0 || warp == 2) {
-        // ---- producers: weights do not wait for the previous kernel, activations do ----
-        if (lane == 0) {
-            const bool wt = warp == 0;
-            if (!wt) pdl_wait();                                          // (nor does any bounded wait span it)
-            const uint8_t *src = w.tiles + ((size_t)rb * w.kblocks + b0) * FP8_TILE_BYTES;
-            int i = 0;
-            for (; i < nb; i++) {
-                const int st = i % S, use = i / S;
-                if (i == S) pdl_wait();
-                if (use > 0 && !wait(&empty[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) break;
-                uint8_t *dst = base + st * Cfg::stage;
-                if (wt) {
-                    mbar_arrive_expect_tx(&full[st], FP8_TILE_BYTES);
-                    bulk_g2s(dst, src + (size_t)i * FP8_TILE_BYTES, FP8_TILE_BYTES, &full[st]);
-                } else {
-                    mbar_arrive_expect_tx(&full[st], NT * FP8_BLOCK);
-                    t5_tma_2d(dst + FP8_TILE_BYTES, &p.tm_q, (b0 + i) * FP8_BLOCK, (int)c0, &full[st]);
-                }
-            }
-            if (*aborted)                                                 // what was issued lands before the CTA ends
-                for (int j = max(0, i - S); j < i; j++) mbar_wait(&full[j % S], (j / S) & 1, nullptr, 0);
-        }
-    } else if (warp == 1) {
-        // ---- products ----
-        pdl_wait();
-        if (lane == 0) {
-            const uint32_t idesc = t5_idesc_e4m3(FP8_BLOCK, NT);
-            for (int i = 0; i < nb; i++) {
-                const int st = i % S, tb = i % B;
-                if (i >= B && !wait(&tempty[tb], (i / B - 1) & 1, FAULT_GEMV_EMPTY)) break;
-                if (!wait(&full[st], (i / S) & 1, FAULT_GEMV_FULL)) break;
-                t5_fence_after();
-                const uint32_t sa = smem_u32(base + st * Cfg::stage), sb = sa + FP8_TILE_BYTES;
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    t5_mma_e4m3(tmem + tb * NT, t5_desc(sa + 32 * k), t5_desc(sb + 32 * k), idesc, k > 0);
-                t5_commit(&empty[st]);
-                t5_commit(&tfull[tb]);
-            }
-            t5_commit(&drain);
-            mbar_wait(&drain, 0, p.fault, FAULT_GEMV_FULL);
-        }
-    } else if (warp == 3) {
-        // ---- scales: activation scale x weight scale, four blocks' loads in flight ----
-        constexpr int L = (NT + 31) / 32;
-        pdl_wait();
-        const float *sw = w.scales + (size_t)rb * w.kblocks + b0;
-        for (int i0 = 0; i0 < nb; i0 += 4) {
-            float v[4][L];
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-#pragma unroll
-                for (int l = 0; l < L; l++) {
-                    const int c = l * 32 + lane;
-                    v[g][l] = i0 + g < nb && c < cols
-                                  ? p.a.s[(c0 + c) * p.a.s_ld + (long long)(b0 + i0 + g) * p.a.s_inc] * sw[i0 + g]
-                                  : 0.f;
-                }
-            bool ok = true;
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int i = i0 + g, sl = i % MMN_SCALE_SLOTS;
-                if (i >= nb) break;
-                ok = ok && (i < MMN_SCALE_SLOTS ||
-                            __all_sync(0xffffffffu, wait(&sempty[sl], (i / MMN_SCALE_SLOTS - 1) & 1, FAULT_GEMV_EMPTY)));
-                if (!ok) break;
-#pragma unroll
-                for (int l = 0; l < L; l++)
-                    if (l * 32 + lane < NT) scales[sl * NT + l * 32 + lane] = v[g][l];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sfull[sl]);
-            }
-            if (!ok) break;
-        }
-    } else {
-        // ---- sums: warp w has tensor-memory lanes 32 * (w % 4) .., half of the columns ----
-        pdl_wait();
-        const int half = (warp - 4) >> 2;
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        for (int i = 0; i < nb; i++) {
-            const int tb = i % B, sl = i % MMN_SCALE_SLOTS;
-            const bool ok = wait(&tfull[tb], (i / B) & 1, FAULT_GEMV_FULL) &&
-                            wait(&sfull[sl], (i / MMN_SCALE_SLOTS) & 1, FAULT_GEMV_FULL);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            t5_fence_after();
-            const float *sc = scales + sl * NT + half * C;
-            constexpr int W = C < 32 ? C : 32;
-#pragma unroll
-            for (int j0 = 0; j0 < C; j0 += W) {
-                uint32_t d[W];
-                t5_ld(tmem + lanes + tb * NT + half * C + j0, d);
-                t5_wait_ld(d);
-#pragma unroll
-                for (int j = 0; j < W; j += 4) {
-                    const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(sc + j0 + j);
-                    acc[(j0 + j) / 2] = t5_fma2(t5_pair(d[j], d[j + 1]), s4.x, acc[(j0 + j) / 2]);
-                    acc[(j0 + j) / 2 + 1] = t5_fma2(t5_pair(d[j + 2], d[j + 3]), s4.y, acc[(j0 + j) / 2 + 1]);
-                }
-            }
-            t5_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&tempty[tb]);
-                mbar_arrive(&sempty[sl]);
-            }
-        }
-    }
-    __syncwarp();
-    __syncthreads();                                                      // the ring is drained: every product is done
-
     TY *y = static_cast<TY *>(p.a.y);
     const int r0 = rb * FP8_BLOCK;
-    if (warp >= 4) {
-        const int half = (warp - 4) >> 2, r = 32 * (warp & 3) + lane;
+    if (warp < 4) {
+        if (Cfg::regs) t5_regs_dec<Cfg::regs_few>();
+        if (warp == 0) {
+            // ---- loads: the first weights do not wait for the previous kernel ----
+            if (lane == 0) {
+                const uint8_t *src = w.tiles + ((size_t)rb * w.kblocks + b0) * FP8_TILE_BYTES;
+                auto load_w = [&](int st, int i) {
+                    mbar_arrive_expect_tx(&full[st], Cfg::stage);
+                    bulk_g2s(base + st * Cfg::stage, src + (size_t)i * FP8_TILE_BYTES, FP8_TILE_BYTES, &full[st]);
+                };
+                auto load_q = [&](int st, int i) {
+                    t5_tma_2d(base + st * Cfg::stage + FP8_TILE_BYTES, &p.tm_q, (b0 + i) * FP8_BLOCK, (int)c0, &full[st]);
+                };
+                const int pre = min(S, nb);
+                for (int i = 0; i < pre; i++) load_w(i, i);
+                pdl_wait();                                                   // (and no bounded wait spans it)
+                for (int i = 0; i < pre; i++) load_q(i, i);
+                int st = 0, par = 0, i = pre;
+                for (; i < nb; i++) {
+                    if (!wait(&done[st], par, FAULT_GEMV_EMPTY)) break;
+                    load_w(st, i);
+                    load_q(st, i);
+                    st++;
+                    par ^= st == S;
+                    st = st == S ? 0 : st;
+                }
+                if (*aborted)                                                 // what was issued lands before the CTA ends
+                    for (int j = max(0, i - S); j < i; j++) mbar_wait(&full[j % S], (j / S) & 1, nullptr, 0);
+            }
+        } else if (warp == 1 || warp == 2) {
+            // ---- products: warp 1 the even blocks, warp 2 the odd ones ----
+            pdl_wait();
+            if (lane == 0) {
+                const uint32_t idesc = t5_idesc_e4m3(FP8_BLOCK, NT), lo = t5_desc_lo(smem_u32(base));
+                int st = warp - 1, par = 0, buf = warp - 1;
+                bool ready = false;                                           // this block's barrier was seen complete
+                for (int i = warp - 1; i < nb; i += 2) {
+                    if (!ready && !wait(&full[st], par, FAULT_GEMV_FULL)) break;
+                    t5_fence_after();
+                    const uint32_t da = lo + st * (Cfg::stage >> 4), db = da + (FP8_TILE_BYTES >> 4), d = tmem + buf * NT;
+                    uint64_t *const f = &done[st];
+                    st += 2;
+                    par ^= st >= S;
+                    st = st >= S ? st - S : st;
+                    buf = (buf + 2) & (B - 1);
+                    ready = mbar_test(&full[st], par);
+                    t5_mma_e4m3<false>(d, da, db, idesc);
+                    t5_mma_e4m3<true>(d, da + 2, db + 2, idesc);
+                    t5_mma_e4m3<true>(d, da + 4, db + 4, idesc);
+                    t5_mma_e4m3<true>(d, da + 6, db + 6, idesc);
+                    t5_commit(f);
+                }
+                t5_commit(&drain);
+            }
+        } else if (warp == 3) {
+            // ---- scales: activation scale x weight scale, a group's loads in flight together ----
+            constexpr int L = (NT + 31) / 32;
+            pdl_wait();
+            const float *sw = w.scales + (size_t)rb * w.kblocks + b0;
+            for (int i0 = 0, gi = 0; i0 < nb; i0 += G, gi++) {
+                float v[G][L];
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int l = 0; l < L; l++) {
+                        const int c = l * 32 + lane;
+                        v[g][l] = i0 + g < nb && c < cols
+                                      ? p.a.s[(c0 + c) * p.a.s_ld + (long long)(b0 + i0 + g) * p.a.s_inc] * sw[i0 + g]
+                                      : 0.f;
+                    }
+                if (gi >= 2 && !__all_sync(0xffffffffu, wait(&sempty[gi & 1], ((gi >> 1) - 1) & 1, FAULT_GEMV_EMPTY))) break;
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int l = 0; l < L; l++)
+                        if (l * 32 + lane < NT) scales[((gi & 1) * G + g) * NT + l * 32 + lane] = v[g][l];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfull[gi & 1]);
+            }
+        }
+        __syncwarp();
+        if (p.ksplit > 1) t5_cluster_sync();                                  // (the summing warps' arrival is what counts)
+    } else {
+        if (Cfg::regs) t5_regs_inc<Cfg::regs_sums>();
+        // ---- sums: warp w has tensor-memory lanes 32 * (w % 4) .., half of the columns ----
+        const int half = (warp - 4) >> 2;
+        const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * C;
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < B; i++) mbar_arrive(&full[i]);            // tensor memory is free
+        pdl_wait();
+        int st = 0, par = 0, buf = 0;
+        bool ok = true;
+        bool arrived = false;                                             // at the cluster's first barrier
+        uint64_t acc[C / 2];                                              // sums of this lane's row, two columns each
+#pragma unroll
+        for (int i = 0; i < C / 2; i++) acc[i] = 0;
+        uint32_t d[2][CH];
+        // Block i, whose first CH columns are on their way to d[F]; before its last are added, the first of block
+        // i + 1 are sent for.
+        auto block = [&](auto first, int i) {
+            constexpr int F = decltype(first)::value;
+            if (i == nb - 1 && p.ksplit > 1) {                             // every product has read its operands
+                t5_cluster_arrive_all();
+                arrived = true;
+            }
+            if (i % G == 0 && !__all_sync(0xffffffffu, wait(&sfull[(i / G) & 1], (i / (2 * G)) & 1, FAULT_GEMV_FULL))) {
+                ok = false;
+                return;
+            }
+            const float *sc = scales + (i % (2 * G)) * NT + half * C;
+            uint64_t *const rel = &full[st + B >= S ? st + B - S : st + B];
+            const uint32_t src = tcol + buf * NT;
+            st++;
+            par ^= st == S;
+            st = st == S ? 0 : st;
+            buf = (buf + 1) & (B - 1);
+            bool ready = __all_sync(0xffffffffu, mbar_test(&done[st], par));
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                uint32_t(&dc)[CH] = d[(F + c) & 1], (&dn)[CH] = d[(F + c + 1) & 1];
+                t5_wait_ld(dc);
+                if (c < NC - 1) {
+                    t5_ld(src + CH * (c + 1), dn);
+                } else {
+                    t5_fence_before();
+                    if (lane == 0) mbar_arrive(rel);
+                    if (i + 1 < nb) {
+                        if (!ready) ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
+                        t5_fence_after();
+                        t5_ld(tcol + buf * NT, dn);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < CH; j += 4) {
+                    const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(sc + CH * c + j);
+                    const int o = (CH * c + j) / 2;
+                    acc[o] = t5_fma2(t5_pair(dc[j], dc[j + 1]), s4.x, acc[o]);
+                    acc[o + 1] = t5_fma2(t5_pair(dc[j + 2], dc[j + 3]), s4.y, acc[o + 1]);
+                }
+            }
+            if (i % G == G - 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sempty[(i / G) & 1]);
+            }
+        };
+        ok = __all_sync(0xffffffffu, wait(&done[0], 0, FAULT_GEMV_FULL));
+        t5_fence_after();
+        t5_ld(tcol, d[0]);
+        for (int i = 0; i < nb && ok; i += 2) {
+            block(std::integral_constant<int, 0>(), i);
+            if (ok && i + 1 < nb) block(std::integral_constant<int, (NC & 1)>(), i + 1);
+        }
+        __syncwarp();
+        if (p.ksplit > 1) {
+            if (!arrived) t5_cluster_arrive_all();
+            t5_cluster_wait_all();
+        }
+        const int r = 32 * (warp & 3) + lane;
         if (p.ksplit == 1) {
             TY *yr = y + (c0 + half * C) * p.a.y_ld + r0 + r;
 #pragma unroll
@@ -248,31 +408,43 @@ __global__ void __launch_bounds__(MMN_THREADS, NT <= 64 ? 2 : 1) k_fp8_mm_n(cons
                 }
             }
         } else {
-            float *part = reinterpret_cast<float *>(base) + (half * C) * FP8_BLOCK + r;
+            // column c is the (c % own)-th of CTA c / own
+            const uint32_t mine = smem_u32(part + (size_t)(ks * p.own) * FP8_BLOCK + r);
+            int o = half * C / p.own, e = half * C % p.own;
 #pragma unroll
-            for (int i = 0; i < C / 2; i++) t5_unpair(acc[i], part[2 * i * FP8_BLOCK], part[(2 * i + 1) * FP8_BLOCK]);
+            for (int i = 0; i < C / 2; i++) {
+                float v[2];
+                t5_unpair(acc[i], v[0], v[1]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (half * C + 2 * i + h < cols) t5_cluster_st(t5_cluster_addr(mine + e * (FP8_BLOCK * 4), o), v[h]);
+                    if (++e == p.own) { e = 0; o++; }
+                }
+            }
         }
     }
+    __syncthreads();
     if (p.ksplit > 1) {
-        // task = (column, 4 rows), dealt over the threads of the cluster's CTAs
         t5_cluster_sync();
-        pdl_wait();
-        const uint32_t part = smem_u32(base);
-        for (int t = ks * MMN_THREADS + tid; t < cols * 32; t += p.ksplit * MMN_THREADS) {
+        // task = (column of this CTA, 4 rows)
+        const int n_own = min(p.own, cols - ks * p.own);
+        for (int t = tid; t < n_own * 32; t += MMN_THREADS) {
             const int col = t >> 5, rq = (t & 31) * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
             for (int s = 0; s < p.ksplit; s++) {
-                const float4 u = t5_cluster_ld4(t5_cluster_addr(part + (col * FP8_BLOCK + rq) * 4, s));
+                const float4 u = *reinterpret_cast<const float4 *>(part + (size_t)(s * p.own + col) * FP8_BLOCK + rq);
                 v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
             }
-            TY *yc = y + (c0 + col) * p.a.y_ld + r0 + rq;
+            TY *yc = y + (c0 + ks * p.own + col) * p.a.y_ld + r0 + rq;
             const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (r0 + rq + j < w.rows) yc[j] = fp8_t<TY>(e[j]);
         }
-        t5_cluster_sync();                                                // the sums stay until every CTA has read them
     }
+    if (tid == 0) mbar_wait(&drain, 0, p.fault, FAULT_GEMV_FULL);
+    __syncthreads();
     if (warp == 1) {
         t5_fence_after();
         t5_dealloc(tmem, Cfg::cols);
@@ -587,8 +759,24 @@ static bool q_map(CUtensorMap *m, const Fp8MmArgs &a, int rows) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launch with programmatic dependent launch and a (1, cluster, 1) cluster; the
-// kernel's attributes are set.
+// Sets kernel k's shared memory once on each device, and checks that it was built
+// with `regs` registers a thread (0: any number).
+template <typename K>
+static cudaError_t kernel_ready(std::atomic<int> (&ready)[64], K k, size_t smem, int regs) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (ready[dev]) return cudaSuccess;
+    cudaFuncAttributes fa = {};
+    e = cudaFuncGetAttributes(&fa, k);
+    if (e == cudaSuccess && regs && fa.numRegs != regs) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) ready[dev] = 1;
+    return e;
+}
+
+// Launch with programmatic dependent launch and a (1, cluster, 1) cluster.
 template <typename P>
 static cudaError_t mm_launch(void (*k)(P), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st,
                              const P &p) {
@@ -609,27 +797,22 @@ static cudaError_t mm_launch(void (*k)(P), dim3 grid, int threads, size_t smem, 
     return cudaLaunchKernelEx(&cfg, k, p);
 }
 
-// Sets kernel k's attributes on the current device; the largest cluster (16, else
-// the portable 8) in which it runs there, 0 on failure.
-template <typename P>
-static int max_cluster(void (*k)(P), int threads, size_t smem) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1, 16);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = 1;
-    at.val.clusterDim.y = 16;
-    at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
-    const bool ok = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-                    cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0;
-    cudaGetLastError();                 // a refused query leaves no error behind
-    return ok ? 16 : 8;
+template <int NG, typename TY>
+static cudaError_t few_launch(const Fp8MmArgs &a, cudaStream_t st) {
+    const int groups = (a.w.rows + 15) / 16;
+    // 32 warps an SM (us at 1, 2, 4, 8, 16 warps a row group: 22016x2048 12.0, 12.5, 10.9, 11.0, 15.8; 2048x11008
+    // 33.6, 16.7, 9.2, 5.3, 4.8; 49152x2048 21.6, 19.7, 19.5, 21.2, 33.1)
+    int kw = 1;
+    while (kw < 16 && (long long)groups * kw < device_sm_count() * 32LL && kw * 2 <= a.w.kblocks) kw *= 2;
+    const int wc = few_warps(kw);
+    const dim3 grid((groups * kw + wc - 1) / wc), block(32 * wc);
+    switch (kw) {
+    case 1: return launch_k(k_fp8_mm_few<NG, 1, TY>, grid, block, 0, st, true, a);
+    case 2: return launch_k(k_fp8_mm_few<NG, 2, TY>, grid, block, 0, st, true, a);
+    case 4: return launch_k(k_fp8_mm_few<NG, 4, TY>, grid, block, 0, st, true, a);
+    case 8: return launch_k(k_fp8_mm_few<NG, 8, TY>, grid, block, 0, st, true, a);
+    default: return launch_k(k_fp8_mm_few<NG, 16, TY>, grid, block, 0, st, true, a);
+    }
 }
 
 template <int NT, typename TY>
@@ -641,16 +824,16 @@ static cudaError_t mmn_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     if (!q_map(&p.tm_q, a, NT)) return cudaErrorInvalidValue;
     const long long tiles = (a.n - 1) / NT + 1;
     // as many CTAs a row block as fill one wave, at least one k block each
-    static std::atomic<int> cluster[64];                                 // per device, 0: not asked yet
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!cluster[dev] && !(cluster[dev] = max_cluster(k_fp8_mm_n<NT, TY>, MMN_THREADS, Cfg::smem)))
-        return cudaErrorInvalidConfiguration;
-    const int slots = device_sm_count() * (NT <= 64 ? 2 : 1);
-    int ks = (int)std::max<long long>(1, std::min<long long>(std::min<int>(cluster[dev], a.w.kblocks), slots / (tiles * a.w.rblocks)));
+    static std::atomic<int> ready[64];
+    const cudaError_t e = kernel_ready(ready, k_fp8_mm_n<NT, TY>, Cfg::smem, Cfg::regs);
+    if (e != cudaSuccess) return e;
+    const int slots = device_sm_count() * Cfg::per_sm;
+    int ks = (int)std::max<long long>(1, std::min<long long>(std::min(MMN_MAX_SPLIT, a.w.kblocks), slots / (tiles * a.w.rblocks)));
+    static const int fks = getenv("KS") ? atoi(getenv("KS")) : 0;
+    if (fks) ks = std::min(ks, fks);
     p.kb_per = (a.w.kblocks + ks - 1) / ks;
     p.ksplit = (a.w.kblocks + p.kb_per - 1) / p.kb_per;
+    p.own = (int)((std::min<long long>(a.n, NT) + p.ksplit - 1) / p.ksplit);
     const dim3 grid((unsigned)tiles, p.ksplit, a.w.rblocks);
     return mm_launch(k_fp8_mm_n<NT, TY>, grid, MMN_THREADS, Cfg::smem, p.ksplit, st, p);
 }
@@ -681,17 +864,8 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     p.vy = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.n == 1 || (a.y_ld * sizeof(TY)) % 16 == 0);
     // the register split of the kernel adds up only to what it was built with
     static std::atomic<int> ready[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!ready[dev]) {
-        cudaFuncAttributes fa = {};
-        cudaError_t e = cudaFuncGetAttributes(&fa, kern);
-        if (e == cudaSuccess && fa.numRegs != MMT_REGS) e = cudaErrorInvalidConfiguration;
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::smem);
-        if (e != cudaSuccess) return e;
-        ready[dev] = 1;
-    }
+    const cudaError_t e = kernel_ready(ready, kern, Cfg::smem, MMT_REGS);
+    if (e != cudaSuccess) return e;
     const long long tiles = (long long)p.mt * p.rt;
     const int pairs = (int)std::min<long long>(tiles, device_sm_count() / 2);
     return launch_k(kern, dim3(2 * pairs), dim3(MMT_THREADS), Cfg::smem, st, true, p);
@@ -735,9 +909,12 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
     const cudaStream_t st = (cudaStream_t)stream;
     CUDA_TRY(fp8_with_type(y_dtype, [&](auto t) {
         using TY = decltype(t);
+        static const int gv = getenv("GV") ? atoi(getenv("GV")) : 16;
+        if (n <= 8 && gv >= n) return few_launch<1, TY>(a, st);
+        if (n <= 16 && gv >= n) return few_launch<2, TY>(a, st);
         if (n <= 16) return mmn_launch<16, TY>(a, fault, st);
         if (n <= 32) return mmn_launch<32, TY>(a, fault, st);
-        if (n <= 64) return mmn_launch<64, TY>(a, fault, st);
+        if (n <= 64 || (getenv("N64") && n<=atoi(getenv("N64")))) return mmn_launch<64, TY>(a, fault, st);
         if (n <= 128) return mmn_launch<128, TY>(a, fault, st);
         return mmt_pick<TY>(a, fault, st);
     }));

@@ -8,15 +8,9 @@
 __device__ __forceinline__ void t5_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void t5_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// K-major operand in shared memory with the 128-byte swizzle: rows of 128
-// bytes, groups of 8 rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t t5_desc(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
-}
-
-// The two words of the same descriptor: the upper does not depend on the
-// address, and 32 bytes further along K is 2 more in the lower.
+// Descriptor of a K-major operand in shared memory with the 128-byte swizzle:
+// rows of 128 bytes, groups of 8 rows 1024 bytes apart.  The upper word does not
+// depend on the address; 32 bytes further along K is 2 more in the lower.
 #define T5_DESC_HI ((1u << 14) | (2u << 29) | (1024u >> 4))
 __device__ __forceinline__ uint32_t t5_desc_lo(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | 1u << 16; }
 
@@ -25,12 +19,15 @@ __host__ __device__ constexpr uint32_t t5_idesc_e4m3(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// D (+)= A . B^T over 32 e4m3 values of K; one thread issues it.
-__device__ __forceinline__ void t5_mma_e4m3(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool acc) {
+// D = A . B^T (ACC: D += A . B^T) over 32 e4m3 values of K; one thread issues it.
+// da, db: lower words of the descriptors.
+template <bool ACC>
+__device__ __forceinline__ void t5_mma_e4m3(uint32_t d, uint32_t da, uint32_t db, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+        "r"(da), "r"(db), "r"(idesc), "n"((int)ACC), "n"(T5_DESC_HI)
         : "memory");
 }
 
@@ -96,23 +93,21 @@ __device__ __forceinline__ void t5_prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
-// Cluster: the address of shared offset `saddr` in CTA `rank`, a 16-byte load
-// from it, and the barrier over all threads of the cluster.
+// Cluster: the address of shared offset `saddr` in CTA `rank`, a store to it, and
+// the barrier over all threads of the cluster.
 __device__ __forceinline__ uint32_t t5_cluster_addr(uint32_t saddr, uint32_t rank) {
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float4 t5_cluster_ld4(uint32_t a) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(a)
-                 : "memory");
-    return v;
+__device__ __forceinline__ void t5_cluster_st(uint32_t a, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
+__device__ __forceinline__ void t5_cluster_arrive_all() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void t5_cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void t5_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    t5_cluster_arrive_all();
+    t5_cluster_wait_all();
 }
 
 // ---- two CTAs of a cluster on one product (cta_group::2) ----
