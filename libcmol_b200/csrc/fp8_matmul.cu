@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(32 * few_warps(KW), KW > 8 ? 1 : 2) k_fp8_mm_f
 #define MMN_THREADS 384
 #define MMN_SUM_WARPS 8
 #define MMN_GROUP 8            // blocks whose scales come together
-#define MMN_MAX_SPLIT 8        // CTAs of a cluster (16 measured slower: 16x2048x11008 15.6 us against 8.5)
+#define MMN_MAX_SPLIT 8        // CTAs of a cluster
 
 struct Fp8MmnArgs {
     CUtensorMap tm_q;          // activations: [n][k] bytes, box 128 x NT, 128-byte swizzle
@@ -171,26 +171,24 @@ struct Fp8MmnArgs {
 
 template <int NT>
 struct MmnCfg {
-    static constexpr int per_sm = NT <= 64 ? 2 : 1;
     // Registers a thread where 32 columns' sums need more than two CTAs an SM leave (0: no split), of the first
     // warpgroup and of the summing warps.
     static constexpr int regs = NT == 64 ? 80 : 0, regs_few = 40, regs_sums = 96;
     static_assert(128 * regs_few + 256 * regs_sums <= 384 * 80, "register split");
     static constexpr int stage = FP8_TILE_BYTES + NT * FP8_BLOCK;
     static constexpr int scales = 2 * MMN_GROUP * NT * 4;
-    static constexpr int stages = ((per_sm == 2 ? 110 : 190) * 1024 - 1024 - scales) / stage / 2 * 2;
-    static constexpr int bufs = NT <= 64 ? 4 : 2;                         // products in tensor memory
-    static constexpr int cols = bufs * NT < 32 ? 32 : bufs * NT;
+    static constexpr int stages = (110 * 1024 - 1024 - scales) / stage / 2 * 2;   // two CTAs an SM
+    static constexpr int bufs = 4, cols = bufs * NT;                      // products in tensor memory
     static constexpr int smem = 1024 + stages * stage + scales;
     static_assert((NT + MMN_MAX_SPLIT) * FP8_BLOCK * 4 <= stages * stage, "ksplit * own columns fit in the ring");
     static_assert(stages >= bufs, "a buffer's release counts on a later block's stage");
 };
 
 template <int NT, typename TY>
-__global__ void __launch_bounds__(MMN_THREADS, MmnCfg<NT>::per_sm) k_fp8_mm_n(const __grid_constant__ Fp8MmnArgs p) {
+__global__ void __launch_bounds__(MMN_THREADS, 2) k_fp8_mm_n(const __grid_constant__ Fp8MmnArgs p) {
     using Cfg = MmnCfg<NT>;
     constexpr int S = Cfg::stages, B = Cfg::bufs, C = NT / 2;             // C: columns of a summing warp
-    constexpr int CH = C < 16 || NT > 64 ? (C < 32 ? C : 32) : 16, NC = C / CH, G = MMN_GROUP;
+    constexpr int CH = C < 16 ? C : 16, NC = C / CH, G = MMN_GROUP;
     const Fp8W &w = p.a.w;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const long long c0 = (long long)blockIdx.x * NT;                      // first activation row
@@ -815,24 +813,29 @@ static cudaError_t few_launch(const Fp8MmArgs &a, cudaStream_t st) {
     }
 }
 
+// CTAs that share k and their blocks each.  Powers of two, and not more than fill
+// most of one wave at two an SM: clusters of six, or of sixteen, left SMs empty
+// (96x2048x11008 at 6: 17.5 us, at 4: 14.4; 16x2048x11008 at 16: 15.6, at 8: 7.3).
+static int mmn_split(const Fp8MmArgs &a, int nt, int &kb_per) {
+    const long long ctas = ((a.n - 1) / nt + 1) * (long long)a.w.rblocks, slots = device_sm_count() * 7LL / 4;
+    int ks = 1;
+    while (ks < MMN_MAX_SPLIT && ks * 2 <= a.w.kblocks && ctas * ks * 2 <= slots) ks *= 2;
+    kb_per = (a.w.kblocks + ks - 1) / ks;
+    return (a.w.kblocks + kb_per - 1) / kb_per;
+}
+
 template <int NT, typename TY>
 static cudaError_t mmn_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
     using Cfg = MmnCfg<NT>;
     Fp8MmnArgs p = {};
     p.a = a;
     p.fault = fault;
-    if (!q_map(&p.tm_q, a, NT)) return cudaErrorInvalidValue;
-    const long long tiles = (a.n - 1) / NT + 1;
-    // as many CTAs a row block as fill one wave, at least one k block each
     static std::atomic<int> ready[64];
     const cudaError_t e = kernel_ready(ready, k_fp8_mm_n<NT, TY>, Cfg::smem, Cfg::regs);
     if (e != cudaSuccess) return e;
-    const int slots = device_sm_count() * Cfg::per_sm;
-    int ks = (int)std::max<long long>(1, std::min<long long>(std::min(MMN_MAX_SPLIT, a.w.kblocks), slots / (tiles * a.w.rblocks)));
-    static const int fks = getenv("KS") ? atoi(getenv("KS")) : 0;
-    if (fks) ks = std::min(ks, fks);
-    p.kb_per = (a.w.kblocks + ks - 1) / ks;
-    p.ksplit = (a.w.kblocks + p.kb_per - 1) / p.kb_per;
+    if (!q_map(&p.tm_q, a, NT)) return cudaErrorInvalidValue;
+    const long long tiles = (a.n - 1) / NT + 1;
+    p.ksplit = mmn_split(a, NT, p.kb_per);
     p.own = (int)((std::min<long long>(a.n, NT) + p.ksplit - 1) / p.ksplit);
     const dim3 grid((unsigned)tiles, p.ksplit, a.w.rblocks);
     return mm_launch(k_fp8_mm_n<NT, TY>, grid, MMN_THREADS, Cfg::smem, p.ksplit, st, p);
@@ -871,16 +874,46 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     return launch_k(kern, dim3(2 * pairs), dim3(MMT_THREADS), Cfg::smem, st, true, p);
 }
 
-// Weight rows of a pair's tile.  A round of 128-row tiles over the pairs of SMs
-// takes 0.62 to 0.72 of one of 256-row tiles (0.33 against 0.47 us a block of 128
-// along k): the narrow ones win where they leave fewer pairs idle (777x2049x8192
-// 32.3 / 47.9 us, 256x22016x2048 20.7 / 22.8, 1000x2048x2048 9.5 / 12.1), the wide
-// ones elsewhere (8192x22016x2048 429 / 370).
+// Which form, by what it is estimated to take (us, from measurements with weights
+// in L2): a fixed part and a block of 128 along k times the blocks that the
+// busiest SM goes through in turn.
+//   k_fp8_mm_n, NT = 16 / 32 / 64:  3.5 + 0.40 / 0.50 / 0.80 a block
+//   k_fp8_mm_t, N = 128 / 256:      3.3 + 0.31 / 0.45 a block, 0.6 / 1.0 a tile
+// Measured, for instance (16, 32, 64 | 128, 256):
+//   64x2048x2048  5.6, 5.9, 6.7 | 7.9, 10.8      64x22016x2048  24.7, 18.5, 17.2 | 19.4, 21.0
+//   128x2048x11008  -, 14.4, 14.3 | 30.1, 41.6   256x22016x2048  -, -, 41.2 | 20.6, 23.0
+//   512x2048x2048  -, -, 11.3 | 8.4, 11.7        2048x22016x2048  -, -, - | 111, 99
+// Up to 16 rows k_fp8_mm_few comes first: always up to 8 (8x2048x2048 2.0 against
+// 4.1, 8x22016x2048 11.5 against 10.7), beyond while the matrix is small, as it reads
+// the activations again for every 16 weight rows (16x5760x960 3.8 against 4.2,
+// 16x11008x2048 8.5 against 6.5).
 template <typename TY>
-static cudaError_t mmt_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
-    const long long mt = (a.n - 1) / 256 + 1, pairs = std::max(1, device_sm_count() / 2);
-    auto rounds = [&](int n) { return (mt * ((a.w.rows - 1) / n + 1) + pairs - 1) / pairs; };
-    return rounds(128) * 62 < rounds(256) * 100 ? mmt_launch<128, TY>(a, fault, st) : mmt_launch<256, TY>(a, fault, st);
+static cudaError_t mm_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
+    if (a.n <= 8) return few_launch<1, TY>(a, st);
+    if (a.n <= 16 && (long long)a.w.rows * a.w.k < 12 << 20) return few_launch<2, TY>(a, st);
+    const int sms = device_sm_count(), nts[3] = {16, 32, 64};
+    const double per[3] = {0.40, 0.50, 0.80};
+    double best = 1e30;
+    int form = 0;
+    for (int i = 0; i < 3; i++) {
+        int kb_per;
+        const long long ks = mmn_split(a, nts[i], kb_per), ctas = ((a.n - 1) / nts[i] + 1) * (long long)a.w.rblocks * ks;
+        const double waves = (double)((ctas + 2 * sms - 1) / (2 * sms)), t = 3.5 + waves * kb_per * per[i] + 2 * (waves - 1);
+        if (t < best) { best = t; form = nts[i]; }
+    }
+    const long long mt = (a.n - 1) / 256 + 1, pairs = std::max(1, sms / 2);
+    for (int n = 128; n <= 256; n += 128) {
+        const long long rounds = (mt * ((a.w.rows - 1) / n + 1) + pairs - 1) / pairs;
+        const double t = 3.3 + rounds * (n == 128 ? a.w.kblocks * 0.31 + 0.6 : a.w.kblocks * 0.45 + 1.0);
+        if (t < best) { best = t; form = n; }
+    }
+    switch (form) {
+    case 16: return mmn_launch<16, TY>(a, fault, st);
+    case 32: return mmn_launch<32, TY>(a, fault, st);
+    case 64: return mmn_launch<64, TY>(a, fault, st);
+    case 128: return mmt_launch<128, TY>(a, fault, st);
+    default: return mmt_launch<256, TY>(a, fault, st);
+    }
 }
 
 extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld, const float *scales,
@@ -908,15 +941,7 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
     unsigned *fault = cmolcu_fault_word(w->device);
     const cudaStream_t st = (cudaStream_t)stream;
     CUDA_TRY(fp8_with_type(y_dtype, [&](auto t) {
-        using TY = decltype(t);
-        static const int gv = getenv("GV") ? atoi(getenv("GV")) : 16;
-        if (n <= 8 && gv >= n) return few_launch<1, TY>(a, st);
-        if (n <= 16 && gv >= n) return few_launch<2, TY>(a, st);
-        if (n <= 16) return mmn_launch<16, TY>(a, fault, st);
-        if (n <= 32) return mmn_launch<32, TY>(a, fault, st);
-        if (n <= 64 || (getenv("N64") && n<=atoi(getenv("N64")))) return mmn_launch<64, TY>(a, fault, st);
-        if (n <= 128) return mmn_launch<128, TY>(a, fault, st);
-        return mmt_pick<TY>(a, fault, st);
+        return mm_pick<decltype(t)>(a, fault, st);
     }));
     return 0;
 }

@@ -273,7 +273,7 @@ def _mm_check(y, q, s, wq, ws):
 MM = [(1, 16, 16), (1, 128, 128), (1, 960, 2560), (2, 300, 960), (1, 2048, 11008), (3, 129, 144), (4, 4096, 576),
       (5, 257, 1040), (8, 2048, 2048), (13, 1000, 1296), (16, 64, 4096), (17, 384, 2064), (31, 2049, 640), (37, 2048, 1100 * 16),
       (64, 515, 2048), (65, 515, 2048), (100, 640, 960), (128, 1536, 576), (129, 256, 256), (200, 2304, 2048),
-      (256, 5000, 1024), (257, 384, 512), (300, 130, 4112), (511, 2560, 960), (777, 641, 1536), (1025, 1281, 400), (2000, 4100, 96),
+      (256, 5000, 1024), (257, 384, 512), (300, 130, 4112), (511, 2560, 960), (777, 641, 1536), (1025, 1281, 400), (2000, 4100, 96), (384, 960, 2560), (130, 2048, 11008),
       (3000, 2500, 2048)]
 
 
