@@ -612,13 +612,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
         pdl_wait();
         int st = 0, par = 0, buf = 0;
         bool ok = true;
-        for (long long t = pair; t < tiles && ok; t += pairs) {
+        const int i1 = min(1, nb - 1);
+        // A tile's first rows, its scales' places and the scales of its first two blocks, which are loaded before the
+        // last tile is written.  Lanes past the last row and warps past the last block sum what they find and write
+        // nothing.
+        struct Tile {
+            long long    row0;                                            // the warp's first activation row
+            int          wrow;                                            // its first weight row
+            const float *sx, *sw;
+            float        x0, w0, x1, w1;
+        };
+        auto tile = [&](long long t) {
+            Tile c;
             const int m = (int)(t % p.mt), r = (int)(t / p.mt);
-            const long long row = (long long)m * 256 + lrow + lane;      // this lane's activation row
-            const int wrow = r * N + half * R, rb = wrow >> 7;            // this warp's first weight row, its block
-            // lanes past the last row and warps past the last block sum what they find and write nothing
-            const float *sx = p.a.s + min(row, (long long)p.a.n - 1) * p.a.s_ld;
-            const float *sw = w.scales + (size_t)min(rb, w.rblocks - 1) * nb;
+            c.row0 = (long long)m * 256 + lrow;
+            c.wrow = r * N + half * R;
+            c.sx = p.a.s + min(c.row0 + lane, (long long)p.a.n - 1) * p.a.s_ld;
+            c.sw = w.scales + (size_t)min(c.wrow >> 7, w.rblocks - 1) * nb;
+            c.x0 = c.sx[0];
+            c.w0 = c.sw[0];
+            c.x1 = c.sx[i1 * p.a.s_inc];
+            c.w1 = c.sw[i1];
+            return c;
+        };
+        Tile nx = tile(pair);
+        for (long long t = pair; t < tiles && ok; t += pairs) {
+            const long long row0 = nx.row0;
+            const int wrow = nx.wrow;
+            const float *sx = nx.sx, *sw = nx.sw;
+            float x0 = nx.x0, w0 = nx.w0, x1 = nx.x1, w1 = nx.w1;
             uint64_t acc[R / 2];
 #pragma unroll
             for (int j = 0; j < R / 2; j++) acc[j] = 0;
@@ -660,8 +682,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                         acc[CH / 2 * c + j] = t5_fma2(t5_pair(dc[2 * j], dc[2 * j + 1]), s2, acc[CH / 2 * c + j]);
                 }
             };
-            const int i1 = min(1, nb - 1);
-            float x0 = sx[0], w0 = sw[0], x1 = sx[i1 * p.a.s_inc], w1 = sw[i1];
             ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
             t5_fence_after();
             t5_ld(tcol + buf * N, d[0]);
@@ -669,7 +689,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                 block(i, x0, w0);
                 if (ok && i + 1 < nb) block(i + 1, x1, w1);
             }
-            if (!ok || rb >= w.rblocks) continue;
+            if (t + pairs < tiles) nx = tile(t + pairs);
+            if (!ok || wrow >= w.rows) continue;
             // ---- out: 64 bytes of each of the warp's 32 rows at a time, through shared memory ----
             constexpr int E = 64 / (int)sizeof(TY), V = 16 / (int)sizeof(TY);   // columns a pass, a 16-byte chunk
             auto place = [&](int lr, int c) { return stg + lr * 64 + ((c ^ ((lr >> 1) & 3)) << 4); };
@@ -689,23 +710,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                     *reinterpret_cast<uint4 *>(place(lane, c)) = *reinterpret_cast<uint4 *>(v);
                 }
                 __syncwarp();
+                const int col0 = wrow + ps * E;
+                if (p.vy && col0 + E <= w.rows) {
 #pragma unroll
-                for (int it = 0; it < 4; it++) {
-                    const int lr = it * 8 + (lane >> 2), ch = lane & 3;
-                    const long long orow = (long long)m * 256 + lrow + lr;
-                    const int ocol = wrow + ps * E + ch * V;
-                    const uint4 v = *reinterpret_cast<const uint4 *>(place(lr, ch));
-                    if (orow < p.a.n) {
-                        TY *o = y + orow * p.a.y_ld + ocol;
-                        if (p.vy && ocol + V <= w.rows) {
-                            *reinterpret_cast<uint4 *>(o) = v;
-                        } else {
-                            const TY *e = reinterpret_cast<const TY *>(&v);
-#pragma unroll
-                            for (int j = 0; j < V; j++)
-                                if (ocol + j < w.rows) o[j] = e[j];
-                        }
+                    for (int it = 0; it < 4; it++) {
+                        const int lr = it * 8 + (lane >> 2), ch = lane & 3;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(place(lr, ch));
+                        if (row0 + lr < p.a.n) *reinterpret_cast<uint4 *>(y + (row0 + lr) * p.a.y_ld + col0 + ch * V) = v;
                     }
+                } else {
+                    // rows at any alignment: consecutive lanes write consecutive values
+                    const int e = lane % E, l0 = lane / E;
+                    if (col0 + e < w.rows)
+#pragma unroll 4
+                        for (int lr = l0; lr < 32 && row0 + lr < p.a.n; lr += 32 / E)
+                            y[(row0 + lr) * p.a.y_ld + col0 + e] = reinterpret_cast<const TY *>(place(lr, e / V))[e % V];
                 }
                 __syncwarp();
             }
@@ -878,7 +897,7 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
 // in L2): a fixed part and a block of 128 along k times the blocks that the
 // busiest SM goes through in turn.
 //   k_fp8_mm_n, NT = 16 / 32 / 64:  3.5 + 0.40 / 0.50 / 0.80 a block
-//   k_fp8_mm_t, N = 128 / 256:      3.3 + 0.31 / 0.45 a block, 0.6 / 1.0 a tile
+//   k_fp8_mm_t, N = 128 / 256:      3.3 + 0.31 / 0.47 a block, 0.6 / 1.5 a tile
 // Measured, for instance (16, 32, 64 | 128, 256):
 //   64x2048x2048  5.6, 5.9, 6.7 | 7.9, 10.8      64x22016x2048  24.7, 18.5, 17.2 | 19.4, 21.0
 //   128x2048x11008  -, 14.4, 14.3 | 30.1, 41.6   256x22016x2048  -, -, 41.2 | 20.6, 23.0
@@ -904,7 +923,7 @@ static cudaError_t mm_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st)
     const long long mt = (a.n - 1) / 256 + 1, pairs = std::max(1, sms / 2);
     for (int n = 128; n <= 256; n += 128) {
         const long long rounds = (mt * ((a.w.rows - 1) / n + 1) + pairs - 1) / pairs;
-        const double t = 3.3 + rounds * (n == 128 ? a.w.kblocks * 0.31 + 0.6 : a.w.kblocks * 0.45 + 1.0);
+        const double t = 3.3 + rounds * (n == 128 ? a.w.kblocks * 0.31 + 0.6 : a.w.kblocks * 0.47 + 1.5);
         if (t < best) { best = t; form = n; }
     }
     switch (form) {
