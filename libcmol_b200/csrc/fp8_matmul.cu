@@ -487,7 +487,7 @@ struct MmtCfg {
     static constexpr int rows = N / 2;                                      // weight rows of a CTA, columns of a sum
     static constexpr int bufs = 512 / N;                                    // products in tensor memory
     static constexpr int stage = FP8_TILE_BYTES + rows * FP8_BLOCK;
-    static constexpr int staging = MMT_SUM_WARPS * 32 * 64;                 // a summing warp's way out: 32 rows x 64 bytes
+    static constexpr int staging = MMT_SUM_WARPS * 2 * 32 * 64;             // a summing warp's way out: twice 32 rows x 64 bytes
     static constexpr int stages = (226 * 1024 - 1024 - staging) / stage / 2 * 2;
     static constexpr int smem = 1024 + stages * stage + staging;
     static_assert(N == 128 || N == 256, "a CTA's rows lie in one row block");
@@ -495,6 +495,7 @@ struct MmtCfg {
 
 struct Fp8MmtArgs {
     CUtensorMap tm_q, tm_w;    // activations as above; weight tiles as rows of 128 bytes
+    CUtensorMap tm_y;          // where vy: y, in boxes of 64 bytes x 32 rows, 64-byte swizzle
     Fp8MmArgs   a;
     int         mt, rt;        // tiles of activation rows and of weight rows
     int         vy;            // rows of y start on 16-byte boundaries
@@ -606,7 +607,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
         const int half = (warp - 4) >> 2, lrow = rank * 128 + 32 * (warp & 3);
         const uint32_t tcol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * R;
         const uint32_t full0 = t5_cluster_addr(smem_u32(&full[0]), 0);   // rank 0's, 8 bytes each
-        uint8_t *stg = base + S * Cfg::stage + (warp - 4) * (32 * 64);
+        uint8_t *const out = base + S * Cfg::stage + (warp - 4) * (2 * 32 * 64);
+        int flip = 0;                                                     // which half of it
 #pragma unroll
         for (int i = 0; i < B; i++) t5_cluster_arrive(full0 + 8 * i, lane == 0);   // tensor memory is free
         pdl_wait();
@@ -693,10 +695,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             if (!ok || wrow >= w.rows) continue;
             // ---- out: 64 bytes of each of the warp's 32 rows at a time, through shared memory ----
             constexpr int E = 64 / (int)sizeof(TY), V = 16 / (int)sizeof(TY);   // columns a pass, a 16-byte chunk
-            auto place = [&](int lr, int c) { return stg + lr * 64 + ((c ^ ((lr >> 1) & 3)) << 4); };
-            TY *y = static_cast<TY *>(p.a.y);
 #pragma unroll
             for (int ps = 0; ps < R / E; ps++) {
+                uint8_t *const stg = out + flip * (32 * 64);
+                auto place = [&](int lr, int c) { return stg + lr * 64 + ((c ^ ((lr >> 1) & 3)) << 4); };
+                flip ^= 1;
+                const int col0 = wrow + ps * E;
+                if (p.vy) {                                               // the copy out of this half, two passes ago
+                    if (lane == 0) t5_tma_store_wait_read<1>();
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     alignas(16) TY v[V];
@@ -709,26 +717,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                     }
                     *reinterpret_cast<uint4 *>(place(lane, c)) = *reinterpret_cast<uint4 *>(v);
                 }
-                __syncwarp();
-                const int col0 = wrow + ps * E;
-                if (p.vy && col0 + E <= w.rows) {
-#pragma unroll
-                    for (int it = 0; it < 4; it++) {
-                        const int lr = it * 8 + (lane >> 2), ch = lane & 3;
-                        const uint4 v = *reinterpret_cast<const uint4 *>(place(lr, ch));
-                        if (row0 + lr < p.a.n) *reinterpret_cast<uint4 *>(y + (row0 + lr) * p.a.y_ld + col0 + ch * V) = v;
+                if (p.vy) {
+                    t5_fence_proxy();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (col0 < w.rows && row0 < p.a.n) t5_tma_store_2d(&p.tm_y, col0, (int)row0, stg);
+                        t5_tma_store_commit();                            // one group a pass, as the wait counts them
                     }
                 } else {
+                    __syncwarp();
                     // rows at any alignment: consecutive lanes write consecutive values
+                    TY *y = static_cast<TY *>(p.a.y);
                     const int e = lane % E, l0 = lane / E;
                     if (col0 + e < w.rows)
 #pragma unroll 4
                         for (int lr = l0; lr < 32 && row0 + lr < p.a.n; lr += 32 / E)
                             y[(row0 + lr) * p.a.y_ld + col0 + e] = reinterpret_cast<const TY *>(place(lr, e / V))[e % V];
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
+        if (p.vy && lane == 0) t5_tma_store_wait_all();
     }
     __syncwarp();
     t5_fence_before();
@@ -873,6 +882,21 @@ static bool w_map(CUtensorMap *m, const Fp8W &w, int rows) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// y, written in boxes of 64 bytes x 32 rows; what lies past it is left alone.
+template <typename TY>
+static bool y_map(CUtensorMap *m, const Fp8MmArgs &a) {
+    const encode_t enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.w.rows, (cuuint64_t)a.n};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.y_ld * sizeof(TY)};
+    const cuuint32_t box[2] = {64 / (cuuint32_t)sizeof(TY), 32}, es[2] = {1u, 1u};
+    const CUtensorMapDataType t = std::is_same<TY, float>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : std::is_same<TY, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return enc(m, t, 2, a.y, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+               CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int N, typename TY>
 static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
     using Cfg = MmtCfg<N>;
@@ -883,7 +907,8 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     if (!q_map(&p.tm_q, a, FP8_BLOCK) || !w_map(&p.tm_w, a.w, Cfg::rows)) return cudaErrorInvalidValue;
     p.mt = (a.n - 1) / 256 + 1;
     p.rt = (a.w.rows - 1) / N + 1;
-    p.vy = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.n == 1 || (a.y_ld * sizeof(TY)) % 16 == 0);
+    p.vy = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.y_ld * sizeof(TY)) % 16 == 0;
+    if (p.vy && !y_map<TY>(&p.tm_y, a)) return cudaErrorInvalidValue;
     // the register split of the kernel adds up only to what it was built with
     static std::atomic<int> ready[64];
     const cudaError_t e = kernel_ready(ready, kern, Cfg::smem, MMT_REGS);

@@ -89,6 +89,24 @@ __device__ __forceinline__ void t5_tma_2d(void *dst, const CUtensorMap *map, int
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
         : "memory");
 }
+// TMA copy of one box from shared memory to (x, y) of `map` (what lies past the
+// tensor is not written): after t5_fence_proxy() by the threads that wrote the
+// box; commit closes a group of the issuing thread's copies (an empty one too), and
+// the waits are for all but the last PENDING groups to have read their boxes, or
+// for all to be done.
+__device__ __forceinline__ void t5_tma_store_2d(const CUtensorMap *map, int x, int y, const void *src) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(smem_u32(src)), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void t5_tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void t5_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void t5_tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PENDING) : "memory"); }
+__device__ __forceinline__ void t5_tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 __device__ __forceinline__ void t5_prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
