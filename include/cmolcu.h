@@ -156,7 +156,9 @@ void cmolcu_matmul_noalloc(float *out, const void *a, const float *b,
  *
  * These calls only launch on `stream` (of `device`, or of the weight's
  * device): they allocate nothing, use no workspace and can be captured.  The
- * calling thread's current device is left as it was.  n = 0 does nothing.
+ * calling thread's current device is left as it was.  n = 0 does nothing.  The
+ * same call gives the same bits; how a sum is split depends on the sizes, so a
+ * row's last bits may differ between calls with different n.
  * Outputs must not overlap inputs, but for res_out = res. */
 #define CMOLCU_BF16 30
 
@@ -203,8 +205,7 @@ size_t cmolcu_fp8_weight_bytes(const cmolcu_fp8_weight_t *w);   /* values and sc
 /* y(c, r) = sum_b sx(c, b) * sw(r/128, b) * sum_{k in b} qx(c, k) * qw(r, k) for
  * n >= 1 activation rows: y is [n][rows] of y_dtype (CMOLCU_F32, _F16 or
  * _BF16), y_ld values apart.  Products and sums in f32, one rounding at the
- * end; the same call gives the same bits.  Waits inside the kernels are
- * bounded (cmolcu_fault_status). */
+ * end.  Waits inside the kernels are bounded (cmolcu_fault_status). */
 int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
                       const float *scales, long long s_ld, long long s_inc, int n,
                       void *y, int y_dtype, long long y_ld, void *stream);

@@ -45,6 +45,18 @@ struct Fp8Device {
     }
 };
 
+// Returns -1 from the calling entry point with the message set when `expr` fails,
+// and leaves no error behind for the program's next look at the runtime's last one.
+#define FP8_TRY(who, expr)                                                      \
+    do {                                                                        \
+        const cudaError_t e_ = (expr);                                          \
+        if (e_ != cudaSuccess) {                                                \
+            cudaGetLastError();                                                 \
+            cmolcu_set_error("%s: %s", who, cudaGetErrorString(e_));            \
+            return -1;                                                          \
+        }                                                                       \
+    } while (0)
+
 // Device fault word of the kernels behind cmolcu.h (seam.cu).
 unsigned int *cmolcu_fault_word(int device);
 

@@ -56,7 +56,7 @@ __device__ __forceinline__ void put(const Fp8Out &o, long long row, int c, const
 // 32 W), V consecutive values a lane and C such chunks; the 128 values of a
 // block are 8 or 16 lanes of one warp, so its amax is three or four shuffles.  A
 // CTA goes through its rows with the next row's loads on their way and the gains
-// in registers.  Rows longer than 12 warps hold (k > 12288) are read twice.
+// in registers.  Rows that are longer (k > 16384; 12288 for f32) are read twice.
 template <typename TX, typename TR, int C>
 struct NormRow {
     static constexpr int  V = lane_values<TX>();
@@ -303,7 +303,7 @@ extern "C" int cmolcu_fp8_rmsnorm(int device, const void *x, int x_dtype, long l
         return -1;
     }
     Fp8Device dev(device);
-    CUDA_TRY(dev.err);
+    FP8_TRY(who, dev.err);
     Fp8ActArgs a = {};
     a.x = x; a.x_ld = x_ld;
     a.r = res; a.r_ld = res_ld;
@@ -315,7 +315,7 @@ extern "C" int cmolcu_fp8_rmsnorm(int device, const void *x, int x_dtype, long l
     a.vg = fp8_vec(norm_w, 0);
     a.o = {static_cast<uint8_t *>(q), q_ld, scales, s_ld, s_inc};
     const cudaStream_t st = (cudaStream_t)stream;
-    CUDA_TRY(fp8_with_type(x_dtype, [&](auto tx) {
+    FP8_TRY(who, fp8_with_type(x_dtype, [&](auto tx) {
         using TX = decltype(tx);
         if (!res) return norm_w ? norm_launch<TX, Fp8None>(a, st) : map_launch<TX, Fp8None, false>(a, st);
         return fp8_with_type(res_dtype, [&](auto tr) {
@@ -336,13 +336,13 @@ extern "C" int cmolcu_fp8_swiglu(int device, const void *gate, long long gate_ld
     if (n == 0) return 0;
     if (!gate || !up) { cmolcu_set_error("%s: NULL argument", who); return -1; }
     Fp8Device dev(device);
-    CUDA_TRY(dev.err);
+    FP8_TRY(who, dev.err);
     Fp8ActArgs a = {};
     a.x = gate; a.x_ld = gate_ld; a.r = up; a.r_ld = up_ld; a.n = n; a.k = k;
     a.vx = fp8_vec(gate, n > 1 ? gate_ld * eb : 0);
     a.vr = fp8_vec(up, n > 1 ? up_ld * eb : 0);
     a.o = {static_cast<uint8_t *>(q), q_ld, scales, s_ld, s_inc};
-    CUDA_TRY(fp8_with_type(dtype, [&](auto t) {
+    FP8_TRY(who, fp8_with_type(dtype, [&](auto t) {
         return map_launch<decltype(t), decltype(t), true>(a, (cudaStream_t)stream);
     }));
     return 0;

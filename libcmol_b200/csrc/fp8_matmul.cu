@@ -976,7 +976,7 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
     }
     if (n > 1 && y_ld < w->w.rows) { cmolcu_set_error("%s: rows of y overlap (y_ld=%lld)", who, y_ld); return -1; }
     Fp8Device dev(w->device);
-    CUDA_TRY(dev.err);
+    FP8_TRY(who, dev.err);
     Fp8MmArgs a = {};
     a.w = w->w;
     a.q = static_cast<const uint8_t *>(q); a.q_ld = q_ld;
@@ -984,7 +984,7 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
     a.n = n; a.y = y; a.y_ld = y_ld;
     unsigned *fault = cmolcu_fault_word(w->device);
     const cudaStream_t st = (cudaStream_t)stream;
-    CUDA_TRY(fp8_with_type(y_dtype, [&](auto t) {
+    FP8_TRY(who, fp8_with_type(y_dtype, [&](auto t) {
         return mm_pick<decltype(t)>(a, fault, st);
     }));
     return 0;

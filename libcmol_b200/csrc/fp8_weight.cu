@@ -79,6 +79,7 @@ static int weight_new(const char *who, int device, int rows, int k, cmolcu_fp8_w
     const size_t nb = (size_t)w.rblocks * w.kblocks;
     cudaError_t e = cudaMalloc(&h->base, nb * (FP8_TILE_BYTES + sizeof(float)));
     if (e != cudaSuccess) {
+        cudaGetLastError();
         cmolcu_set_error("%s: %s", who, cudaGetErrorString(e));
         delete h;
         return -1;
@@ -108,6 +109,7 @@ static int weight_done(const char *who, cudaError_t e, cudaStream_t st, cmolcu_f
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e == cudaSuccess && !cmolcu_fault_word(h->device)) e = cudaErrorMemoryAllocation;   // the product's, made here
     if (e != cudaSuccess) {
+        cudaGetLastError();
         cmolcu_set_error("%s: %s", who, cudaGetErrorString(e));
         cmolcu_fp8_weight_free(h);
         return -1;
@@ -132,7 +134,7 @@ extern "C" int cmolcu_fp8_weight_upload(int device, const void *q, const float *
     if (shape_check(who, q, rows, k, k, out)) return -1;
     if (!scales) { cmolcu_set_error("%s: NULL argument", who); return -1; }
     Fp8Device dev(device);
-    CUDA_TRY(dev.err);
+    FP8_TRY(who, dev.err);
     cmolcu_fp8_weight_t *h = nullptr;
     if (weight_new(who, device, rows, k, &h)) return -1;
     void *tmp = nullptr;
@@ -154,7 +156,7 @@ extern "C" int cmolcu_fp8_weight_upload_dev(int device, const void *q, long long
         return -1;
     }
     Fp8Device dev(device);
-    CUDA_TRY(dev.err);
+    FP8_TRY(who, dev.err);
     cmolcu_fp8_weight_t *h = nullptr;
     if (weight_new(who, device, rows, k, &h)) return -1;
     const cudaError_t e = tile_launch(q, q_ld, scales, cudaMemcpyDeviceToDevice, h, (cudaStream_t)stream);
@@ -168,7 +170,7 @@ extern "C" int cmolcu_fp8_weight_quantize_dev(int device, const void *w, int dty
     const int eb = fp8_elem_bytes(dtype);
     if (!eb) { cmolcu_set_error("%s: unsupported dtype %d", who, dtype); return -1; }
     Fp8Device dev(device);
-    CUDA_TRY(dev.err);
+    FP8_TRY(who, dev.err);
     cmolcu_fp8_weight_t *h = nullptr;
     if (weight_new(who, device, rows, k, &h)) return -1;
     const int vec = fp8_vec(w, ld * eb);
@@ -191,10 +193,10 @@ extern "C" int cmolcu_fp8_weight_read_dev(const cmolcu_fp8_weight_t *h, void *q,
         return -1;
     }
     Fp8Device dev(h->device);
-    CUDA_TRY(dev.err);
-    CUDA_TRY(cudaMemcpyAsync(scales, w.scales, (size_t)w.rblocks * w.kblocks * sizeof(float),
+    FP8_TRY(who, dev.err);
+    FP8_TRY(who, cudaMemcpyAsync(scales, w.scales, (size_t)w.rblocks * w.kblocks * sizeof(float),
                              cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
-    CUDA_TRY(launch_k(k_fp8_untile, dim3(w.kblocks, w.rblocks), dim3(256), 0, (cudaStream_t)stream, false, w,
+    FP8_TRY(who, launch_k(k_fp8_untile, dim3(w.kblocks, w.rblocks), dim3(256), 0, (cudaStream_t)stream, false, w,
                       static_cast<uint8_t *>(q), q_ld));
     return 0;
 }

@@ -495,3 +495,136 @@ def test_current_device_is_left_alone_and_no_fault():
     assert torch.cuda.current_device() == 0
     code = C.c_uint(0)
     assert lib().cmolcu_fault_status(0, C.byref(code), 0) == 0 and code.value == 0
+
+
+# ---------------------------------------------------------------------------
+# Calls that the documentation allows and an ordinary program seldom makes
+# ---------------------------------------------------------------------------
+def test_the_residual_may_be_the_input():
+    """h = x + x, written back over x: short and long rows."""
+    from libcmol_b200 import fp8
+    for n, k in [(300, 960), (3, 20000)]:
+        g = _gen(k)
+        x, w = _randn(g, n, k), 1 + 0.1 * _randn(g, k)
+        x0 = x.clone()
+        q, s = fp8.rmsnorm(x, w, 1e-5, residual=x)
+        h, v = _norm_ref(x0, x0, w, 1e-5)
+        assert torch.equal(x.double(), h)
+        _check_eight_bits(v, q, s, _norm_delta(k))
+
+
+def test_rows_with_nan_among_many():
+    """A NaN stays in its row where a CTA goes through several rows."""
+    from libcmol_b200 import fp8
+    g = _gen(9)
+    n, k = 5000, 960
+    x, w = _randn(g, n, k, dtype=BF16), 1 + 0.1 * _randn(g, k)
+    bad = [0, 17, 2500, n - 1]
+    x[bad, 3] = float("nan")
+    q, s = fp8.rmsnorm(x, w, 1e-5)
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[bad] = False
+    assert torch.isnan(s[bad]).all()
+    _check_eight_bits(_norm_ref(x[good], None, w, 1e-5)[1], q[good], s[good], _norm_delta(k))
+
+
+def test_a_wrong_device_is_refused_and_leaves_no_error():
+    from libcmol_b200 import last_error, lib
+    x = torch.zeros(16, device="cuda")
+    p = x.data_ptr()
+    assert lib().cmolcu_fp8_rmsnorm(97, p, 0, 16, None, 0, None, 0, 0, None, 0.0, 1, 16, p, 16, p, 1, 1, None) == -1
+    assert "cmolcu_fp8_rmsnorm" in last_error()
+    assert (x + 1 == 1).all() and torch.cuda.current_device() == 0
+
+
+def test_first_use_inside_a_capture():
+    """Nothing has to run before a capture but the making of the weight."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from libcmol_b200 import fp8
+W = [fp8.Fp8Weight.quantize(torch.randn(r, 1024, device="cuda")) for r in (256, 24000)]
+x = [torch.randn(n, 1024, device="cuda") for n in (1, 12, 40, 600)]
+w = torch.ones(1024, device="cuda")
+def go():
+    out = []
+    for a in x:
+        q, s = fp8.rmsnorm(a, w, 1e-5)
+        q2, s2 = fp8.swiglu(a, a)
+        out += [W[0].matmul(q, s), W[1].matmul(q, s, dtype=torch.bfloat16), W[0].matmul(q2, s2, dtype=torch.float16)]
+    return out
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = go()
+g.replay()
+torch.cuda.synchronize()
+want = go()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+def test_threads_share_a_weight():
+    import threading
+    from libcmol_b200 import fp8
+    g = _gen(12)
+    W = fp8.Fp8Weight.quantize(_weight(g, 640, 512))
+    ins = [_acts(g, n, 512) for n in (1, 14, 50, 700)]
+    want = [W.matmul(q, s) for q, s in ins]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                y = W.matmul(*ins[i])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[i]):
+                    wrong.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not wrong
+
+
+def test_offsets_past_32_bits():
+    """Activations, outputs and a weight of more than 2^32 bytes: what lies at the
+    end."""
+    from libcmol_b200 import fp8
+    g = _gen(13)
+    n, k = 2_200_003, 1024                       # x: 4.5 GB, q: 2.25 GB
+    x = torch.zeros(n, k, dtype=BF16, device="cuda")
+    x[-300:] = _randn(g, 300, k, dtype=BF16)
+    w = 1 + 0.1 * _randn(g, k)
+    q, s = fp8.rmsnorm(x, w, 1e-5)
+    q1, s1 = q[-300:].clone(), s[-300:].clone()
+    _check_eight_bits(_norm_ref(x[-300:], None, w, 1e-5)[1], q1, s1, _norm_delta(k))
+    assert (q[:1000].double() == 0).all()
+    del x
+    W = fp8.Fp8Weight.quantize(_weight(g, 600, k))
+    y = W.matmul(q, s, dtype=F32)                # 5.3 GB
+    assert (y[:1000] == 0).all()
+    _mm_check(y[-300:], q1, s1, *W.read())
+    del q, s, y
+    torch.cuda.empty_cache()
+    rows, k = 1_100_033, 4096                    # 4.5 GB
+    wq = torch.zeros(rows, k, dtype=torch.uint8, device="cuda")
+    tail = (100 * _randn(g, 161, k)).clamp(-448, 448).to(E4M3)
+    wq[-161:] = tail.view(torch.uint8)           # the last two row blocks: 128 + 33
+    ws = torch.ones(-(-rows // 128), k // 128, device="cuda")
+    W = fp8.Fp8Weight(wq.view(E4M3), ws)
+    del wq
+    for n in (2, 40, 300):
+        q, s = _acts(g, n, k)
+        y = W.matmul(q, s)
+        _mm_check(y[:, -161:], q, s, tail, torch.ones(2, k // 128, device="cuda"))
+        assert (y[:, :1000] == 0).all()
+        del y
+    W.free()
