@@ -485,8 +485,9 @@ static_assert(128 * MMT_REGS_FEW + 32 * MMT_SUM_WARPS * MMT_REGS_SUMS == MMT_THR
 template <int N>
 struct MmtCfg {
     static constexpr int rows = N / 2;                                      // weight rows of a CTA, columns of a sum
-    static constexpr int bufs = 512 / N;                                    // products in tensor memory
-    static constexpr int stage = FP8_TILE_BYTES + rows * FP8_BLOCK;
+    static constexpr int group = 256 / N;                                   // blocks along k between two barriers
+    static constexpr int block = FP8_TILE_BYTES + rows * FP8_BLOCK;
+    static constexpr int stage = group * block;
     static constexpr int staging = MMT_SUM_WARPS * 2 * 32 * 64;             // a summing warp's way out: twice 32 rows x 64 bytes
     static constexpr int stages = (226 * 1024 - 1024 - staging) / stage / 2 * 2;
     static constexpr int smem = 1024 + stages * stage + staging;
@@ -505,14 +506,14 @@ struct Fp8MmtArgs {
 template <int N, typename TY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp8_mm_t(const __grid_constant__ Fp8MmtArgs p) {
     using Cfg = MmtCfg<N>;
-    constexpr int S = Cfg::stages, B = Cfg::bufs, R = Cfg::rows, CH = 32, NC = R / CH;
+    constexpr int S = Cfg::stages, B = 2, G = Cfg::group, R = Cfg::rows, CH = 32, NC = 128 / CH;
     static_assert(S % 2 == 0, "a stage belongs to one of the two issuing warps");
     const Fp8W &w = p.a.w;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)t5_cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const long long tiles = (long long)p.mt * p.rt;
-    const int nb = w.kblocks;
+    const int nb = w.kblocks, nr = (nb + G - 1) / G;    // blocks and groups of blocks along k
 
     uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)cmolcu_smem + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[S], done[S], drain;        // full: rank 0's counts
@@ -556,7 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             for (long long t = pair; t < tiles && ok; t += pairs) {
                 const int m = (int)(t % p.mt), r = (int)(t / p.mt);
                 const int row = m * 256 + rank * 128, wrow = r * N + rank * R;
-                for (int i = 0; i < nb; i++) {
+                for (int i = 0; i < nr; i++) {
                     if (use > 0 && !wait(&done[st], (use - 1) & 1, FAULT_GEMV_EMPTY)) {
                         ok = false;
                         break;
@@ -564,8 +565,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                     uint8_t *dst = base + st * Cfg::stage;
                     if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * Cfg::stage);
                     const uint32_t bar = t5_cluster_addr(smem_u32(&full[st]), 0);
-                    t5_tma2_2d(dst, &p.tm_q, i * FP8_BLOCK, row, bar);
-                    t5_tma2_2d(dst + FP8_TILE_BYTES, &p.tm_w, 0, ((wrow >> 7) * nb + i) * FP8_BLOCK + (wrow & 127), bar);
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        // a block past the last: both operands lie past their tensors and read as zero
+                        const int b = i * G + g, rb = b < nb ? wrow >> 7 : w.rblocks;
+                        t5_tma2_2d(dst + g * Cfg::block, &p.tm_q, b * FP8_BLOCK, row, bar);
+                        t5_tma2_2d(dst + g * Cfg::block + FP8_TILE_BYTES, &p.tm_w, 0,
+                                   (rb * nb + (b < nb ? b : 0)) * FP8_BLOCK + (wrow & 127), bar);
+                    }
                     if (++st == S) { st = 0; use++; }
                 }
             }
@@ -575,28 +582,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                     if (u >= 0) mbar_wait(&full[j], u & 1, nullptr, 0);
                 }
         } else if ((warp & 1) && lane == 0 && rank == 0) {
-            // ---- products: warp 1 the even blocks, warp 3 the odd ones ----
+            // ---- products: warp 1 the even groups, warp 3 the odd ones ----
             pdl_wait();                         // so that no bounded wait spans the previous kernel
             const uint32_t idesc = t5_idesc_e4m3(256, N);
             const uint32_t lo = t5_desc_lo(smem_u32(base));
-            const long long blocks = (tiles - pair + pairs - 1) / pairs * nb;
-            int st = warp >> 1, par = 0, buf = warp >> 1;
-            bool ready = false;                 // this block's barrier was seen complete in the last round
-            for (long long j = warp >> 1; j < blocks; j += 2) {
+            const long long groups = (tiles - pair + pairs - 1) / pairs * nr;
+            const uint32_t d = tmem + (warp >> 1) * 256;
+            int st = warp >> 1, par = 0;
+            bool ready = false;                 // this group's barrier was seen complete in the last round
+            for (long long j = warp >> 1; j < groups; j += 2) {
                 if (!ready && !wait(&full[st], par, FAULT_GEMV_FULL)) break;
                 t5_fence_after();
-                const uint32_t da = lo + st * (Cfg::stage >> 4), db = da + (FP8_TILE_BYTES >> 4);
-                const uint32_t d = tmem + buf * N;
+                const uint32_t a0 = lo + st * (Cfg::stage >> 4);
                 uint64_t *const f = &done[st];
                 st += 2;
                 par ^= st >= S;
                 st = st >= S ? st - S : st;
-                buf = buf + 2 >= B ? buf + 2 - B : buf + 2;
                 ready = mbar_test(&full[st], par);
-                t5_mma2_e4m3<false>(d, da, db, idesc);
-                t5_mma2_e4m3<true>(d, da + 2, db + 2, idesc);
-                t5_mma2_e4m3<true>(d, da + 4, db + 4, idesc);
-                t5_mma2_e4m3<true>(d, da + 6, db + 6, idesc);
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    const uint32_t da = a0 + g * (Cfg::block >> 4), db = da + (FP8_TILE_BYTES >> 4);
+                    t5_mma2_e4m3<false>(d + g * N, da, db, idesc);
+                    t5_mma2_e4m3<true>(d + g * N, da + 2, db + 2, idesc);
+                    t5_mma2_e4m3<true>(d + g * N, da + 4, db + 4, idesc);
+                    t5_mma2_e4m3<true>(d + g * N, da + 6, db + 6, idesc);
+                }
                 t5_commit2(f);
             }
             t5_commit2(&drain);
@@ -614,15 +624,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
         pdl_wait();
         int st = 0, par = 0, buf = 0;
         bool ok = true;
-        const int i1 = min(1, nb - 1);
-        // A tile's first rows, its scales' places and the scales of its first two blocks, which are loaded before the
+        // A tile's first rows, its scales' places and the scales of its first two groups, which are loaded before the
         // last tile is written.  Lanes past the last row and warps past the last block sum what they find and write
         // nothing.
         struct Tile {
             long long    row0;                                            // the warp's first activation row
             int          wrow;                                            // its first weight row
             const float *sx, *sw;
-            float        x0, w0, x1, w1;
+            float        x[2][G], w[2][G];
         };
         auto tile = [&](long long t) {
             Tile c;
@@ -631,10 +640,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             c.wrow = r * N + half * R;
             c.sx = p.a.s + min(c.row0 + lane, (long long)p.a.n - 1) * p.a.s_ld;
             c.sw = w.scales + (size_t)min(c.wrow >> 7, w.rblocks - 1) * nb;
-            c.x0 = c.sx[0];
-            c.w0 = c.sw[0];
-            c.x1 = c.sx[i1 * p.a.s_inc];
-            c.w1 = c.sw[i1];
+#pragma unroll
+            for (int j = 0; j < 2 * G; j++) {
+                const int b = min(j, nb - 1);
+                c.x[j / G][j % G] = c.sx[b * p.a.s_inc];
+                c.w[j / G][j % G] = c.sw[b];
+            }
             return c;
         };
         Tile nx = tile(pair);
@@ -642,54 +653,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             const long long row0 = nx.row0;
             const int wrow = nx.wrow;
             const float *sx = nx.sx, *sw = nx.sw;
-            float x0 = nx.x0, w0 = nx.w0, x1 = nx.x1, w1 = nx.w1;
+            float x[2][G], ws[2][G];
+#pragma unroll
+            for (int j = 0; j < 2 * G; j++) {
+                x[j / G][j % G] = nx.x[j / G][j % G];
+                ws[j / G][j % G] = nx.w[j / G][j % G];
+            }
             uint64_t acc[R / 2];
 #pragma unroll
             for (int j = 0; j < R / 2; j++) acc[j] = 0;
             uint32_t d[2][CH];
-            // Block i, whose first 32 columns are on their way to d[0]; before its last 32 are added, the first of
-            // block i + 1 are sent for.  x and ws, its scales, were loaded two blocks ago and their place takes those
-            // of block i + 2.
-            auto block = [&](int i, float &x, float &ws) {
-                const float s = x * ws;
-                const uint64_t s2 = t5_pair(__float_as_uint(s), __float_as_uint(s));
-                const int i2 = min(i + 2, nb - 1);
-                x = sx[i2 * p.a.s_inc];
-                ws = sw[i2];
-                // released for the block B blocks on, which waits for this on its stage's barrier
-                const uint32_t rel = full0 + 8 * (st + B >= S ? st + B - S : st + B), src = tcol + buf * N;
+            // Group i of blocks, whose first 32 columns are on their way to d[0]; before its last 32 are added, the
+            // first of group i + 1 are sent for.  xg and wg, its scales, were loaded two groups ago and their place
+            // takes those of group i + 2.
+            auto group = [&](int i, float (&xg)[G], float (&wg)[G]) {
+                uint64_t s2[G];
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    const float s = i * G + g < nb ? xg[g] * wg[g] : 0.f;
+                    s2[g] = t5_pair(__float_as_uint(s), __float_as_uint(s));
+                    const int b = min((i + 2) * G + g, nb - 1);
+                    xg[g] = sx[b * p.a.s_inc];
+                    wg[g] = sw[b];
+                }
+                // released for the group B groups on, which waits for this on its stage's barrier
+                const uint32_t rel = full0 + 8 * (st + B >= S ? st + B - S : st + B), src = tcol + buf * 256;
                 st++;
                 par ^= st == S;
                 st = st == S ? 0 : st;
-                buf = buf + 1 == B ? 0 : buf + 1;
+                buf ^= 1;
                 bool ready = false;
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     uint32_t(&dc)[CH] = d[c & 1], (&dn)[CH] = d[(c + 1) & 1];
                     t5_wait_ld(dc);
                     if (c < NC - 1) {
-                        t5_ld(src + CH * (c + 1), dn);
+                        t5_ld(src + (c + 1) * CH / R * N + (c + 1) * CH % R, dn);
                         if (c == NC - 2) ready = __all_sync(0xffffffffu, mbar_test(&done[st], par));
                     } else {
                         t5_fence_before();
                         t5_cluster_arrive(rel, lane == 0);
-                        if (i + 1 < nb) {
+                        if (i + 1 < nr) {
                             if (!ready) ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
                             t5_fence_after();
-                            t5_ld(tcol + buf * N, dn);
+                            t5_ld(tcol + buf * 256, dn);
                         }
                     }
 #pragma unroll
                     for (int j = 0; j < CH / 2; j++)
-                        acc[CH / 2 * c + j] = t5_fma2(t5_pair(dc[2 * j], dc[2 * j + 1]), s2, acc[CH / 2 * c + j]);
+                        acc[c * CH % R / 2 + j] =
+                            t5_fma2(t5_pair(dc[2 * j], dc[2 * j + 1]), s2[c * CH / R], acc[c * CH % R / 2 + j]);
                 }
             };
             ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
             t5_fence_after();
-            t5_ld(tcol + buf * N, d[0]);
-            for (int i = 0; i < nb && ok; i += 2) {
-                block(i, x0, w0);
-                if (ok && i + 1 < nb) block(i + 1, x1, w1);
+            t5_ld(tcol + buf * 256, d[0]);
+            for (int i = 0; i < nr && ok; i += 2) {
+                group(i, x[0], ws[0]);
+                if (ok && i + 1 < nr) group(i + 1, x[1], ws[1]);
             }
             if (t + pairs < tiles) nx = tile(t + pairs);
             if (!ok || wrow >= w.rows) continue;
@@ -921,12 +942,12 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
 // Which form, by what it is estimated to take (us, from measurements with weights
 // in L2): a fixed part and a block of 128 along k times the blocks that the
 // busiest SM goes through in turn.
-//   k_fp8_mm_n, NT = 16 / 32 / 64:  3.5 + 0.40 / 0.50 / 0.80 a block
-//   k_fp8_mm_t, N = 128 / 256:      3.3 + 0.31 / 0.47 a block, 0.6 / 1.5 a tile
-// Measured, for instance (16, 32, 64 | 128, 256):
-//   64x2048x2048  5.6, 5.9, 6.7 | 7.9, 10.8      64x22016x2048  24.7, 18.5, 17.2 | 19.4, 21.0
-//   128x2048x11008  -, 14.4, 14.3 | 30.1, 41.6   256x22016x2048  -, -, 41.2 | 20.6, 23.0
-//   512x2048x2048  -, -, 11.3 | 8.4, 11.7        2048x22016x2048  -, -, - | 111, 99
+//   k_fp8_mm_n, NT = 16 / 32 / 64:  3.5 (4.3 at two CTAs an SM) + 0.40 / 0.50 / 0.80 a block
+//   k_fp8_mm_t, N = 128 / 256:      3.3 + 0.25 / 0.47 a block, 0.5 / 1.5 a tile
+// Measured, for instance (32, 64 | 128, 256):
+//   64x2048x2048  6.1, 6.8 | 7.0, 11.2      64x22016x2048  18.7, 17.3 | 17.5, 21.5
+//   128x2048x11008  14.4, 14.2 | 23.4, 42.3   256x22016x2048  -, 42.2 | 18.3, 22.6
+//   512x2048x2048  -, 11.3 | 7.5, 11.6        2048x22016x2048  -, - | 100, 97
 // Up to 16 rows k_fp8_mm_few comes first: always up to 8 (8x2048x2048 2.0 against
 // 4.1, 8x22016x2048 11.5 against 10.7), beyond while the matrix is small, as it reads
 // the activations again for every 16 weight rows (16x5760x960 3.8 against 4.2,
@@ -942,13 +963,13 @@ static cudaError_t mm_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st)
     for (int i = 0; i < 3; i++) {
         int kb_per;
         const long long ks = mmn_split(a, nts[i], kb_per), ctas = ((a.n - 1) / nts[i] + 1) * (long long)a.w.rblocks * ks;
-        const double waves = (double)((ctas + 2 * sms - 1) / (2 * sms)), t = 3.5 + waves * kb_per * per[i] + 2 * (waves - 1);
+        const double waves = (double)((ctas + 2 * sms - 1) / (2 * sms)), t = (ctas > sms ? 4.3 : 3.5) + waves * kb_per * per[i] + 2 * (waves - 1);
         if (t < best) { best = t; form = nts[i]; }
     }
     const long long mt = (a.n - 1) / 256 + 1, pairs = std::max(1, sms / 2);
     for (int n = 128; n <= 256; n += 128) {
         const long long rounds = (mt * ((a.w.rows - 1) / n + 1) + pairs - 1) / pairs;
-        const double t = 3.3 + rounds * (n == 128 ? a.w.kblocks * 0.31 + 0.6 : a.w.kblocks * 0.47 + 1.5);
+        const double t = 3.3 + rounds * (n == 128 ? a.w.kblocks * 0.25 + 0.5 : a.w.kblocks * 0.47 + 1.5);
         if (t < best) { best = t; form = n; }
     }
     switch (form) {
