@@ -123,10 +123,39 @@ inline int fp8_vec(const void *p, long long ld_bytes) {
     return a % 32 == 0 ? 2 : a % 16 == 0 ? 1 : 0;
 }
 
-// max(a, |b|) that keeps a NaN of either side.
+// Two f32 operations in one instruction: the activation kernels stream memory
+// under the power limit, where instructions cost clock.
+__device__ __forceinline__ float2 fp8_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fp8_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fp8_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// max(a, |b|) and max(a, |b|, |c|) that keep a NaN of any side (a >= 0).
 __device__ __forceinline__ float fp8_amax(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+__device__ __forceinline__ float fp8_amax(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -153,8 +182,13 @@ __device__ __forceinline__ uint32_t fp8_pack2(float lo, float hi) {
 }
 
 __device__ __forceinline__ uint2 fp8_pack8(const float v[8], float inv) {
-    return make_uint2(fp8_pack2(v[0] * inv, v[1] * inv) | fp8_pack2(v[2] * inv, v[3] * inv) << 16,
-                      fp8_pack2(v[4] * inv, v[5] * inv) | fp8_pack2(v[6] * inv, v[7] * inv) << 16);
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 p = fp8_mul2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(inv, inv));
+        h[i] = fp8_pack2(p.x, p.y);
+    }
+    return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
 // V e4m3 values to consecutive bytes (V-byte aligned).
@@ -173,7 +207,7 @@ template <int V>
 __device__ __forceinline__ float fp8_block_amax(const float v[V]) {
     float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; i++) a = fp8_amax(a, v[i]);
+    for (int i = 0; i < V; i += 2) a = fp8_amax(a, v[i], v[i + 1]);
 #pragma unroll
     for (int o = FP8_BLOCK / V / 2; o > 0; o >>= 1) a = fp8_amax(a, __shfl_xor_sync(0xffffffffu, a, o));
     return a;

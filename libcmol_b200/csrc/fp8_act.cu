@@ -56,7 +56,8 @@ __device__ __forceinline__ void put(const Fp8Out &o, long long row, int c, const
 // 32 W), V consecutive values a lane and C such chunks; the 128 values of a
 // block are 8 or 16 lanes of one warp, so its amax is three or four shuffles.  A
 // CTA goes through its rows with the next row's loads on their way and the gains
-// in registers.  Rows that are longer (k > 16384; 12288 for f32) are read twice.
+// in registers.  Rows that are longer (k > 16384; 12288 with f32
+// values) are read twice.
 template <typename TX, typename TR, int C>
 struct NormRow {
     static constexpr int  V = lane_values<TX>();
@@ -84,9 +85,11 @@ struct NormRow {
 #pragma unroll
         for (int i = 0; i < C; i++)
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                v[i][e] = fp8_f(x[i].e[e]);
-                if constexpr (RES) v[i][e] += fp8_f(r[i].e[e]);
+            for (int e = 0; e < V; e += 2) {
+                float2 h = make_float2(fp8_f(x[i].e[e]), fp8_f(x[i].e[e + 1]));
+                if constexpr (RES) h = fp8_add2(h, make_float2(fp8_f(r[i].e[e]), fp8_f(r[i].e[e + 1])));
+                v[i][e] = h.x;
+                v[i][e + 1] = h.y;
             }
     }
     __device__ __forceinline__ static void store_sum(const Fp8ActArgs &a, long long row, int c, const float (&v)[V]) {
@@ -98,6 +101,28 @@ struct NormRow {
         }
     }
 };
+
+// ss + the squares of v.
+template <int V>
+__device__ __forceinline__ float2 squares(float2 ss, const float (&v)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+        const float2 h = make_float2(v[e], v[e + 1]);
+        ss = fp8_fma2(h, h, ss);
+    }
+    return ss;
+}
+
+// v = g * (v * ir)
+template <int V>
+__device__ __forceinline__ void normalise(float (&v)[V], const float *g, float ir) {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+        const float2 h = fp8_mul2(make_float2(g[e], g[e + 1]), fp8_mul2(make_float2(v[e], v[e + 1]), make_float2(ir, ir)));
+        v[e] = h.x;
+        v[e + 1] = h.y;
+    }
+}
 
 // Sum over the T threads of a row; red: a float a warp, of this row's own.
 __device__ __forceinline__ float row_sum(float v, int T, float *red) {
@@ -112,16 +137,19 @@ __device__ __forceinline__ float row_sum(float v, int T, float *red) {
 }
 
 // Most warps a row: the chunks a lane holds bound the threads that the registers allow.
-static constexpr int norm_warps(int c) { return c == 1 ? 24 : c == 2 ? 16 : 12; }
+template <typename TX, typename TR>
+constexpr int norm_warps(int c) {
+    return c == 1 ? 24 : c == 2 && !(sizeof(TX) == 2 && std::is_same<TR, float>::value) ? 16 : 12;
+}
 
 template <typename TX, typename TR, int C>
-__global__ void __launch_bounds__(32 * norm_warps(C)) k_fp8_norm(const Fp8ActArgs a) {
+__global__ void __launch_bounds__(32 * norm_warps<TX, TR>(C)) k_fp8_norm(const Fp8ActArgs a) {
     using Row = NormRow<TX, TR, C>;
     constexpr int V = Row::V;
     const int T = blockDim.x, t = threadIdx.x, nchunk = a.k / V;
     const long long step = (long long)gridDim.x * blockDim.y;
     long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-    __shared__ float red[2][norm_warps(C)];
+    __shared__ float red[2][norm_warps<TX, TR>(C)];
     int flip = 0;
     pdl_wait();
     pdl_launch_dependents();
@@ -134,14 +162,13 @@ __global__ void __launch_bounds__(32 * norm_warps(C)) k_fp8_norm(const Fp8ActArg
         if (i * T + t < nchunk) g[i].load(a.g + (long long)(i * T + t) * V, a.vg);
     }
     for (; row < a.n; row += step) {                        // the rows of a CTA with several warps a row: all or none
-        float v[C][V], ss = 0.f;
+        float v[C][V];
+        float2 ss2 = make_float2(0.f, 0.f);
         x.sum(v);
         if (row + step < a.n) x.load(a, row + step, t, T);
 #pragma unroll
-        for (int i = 0; i < C; i++)
-#pragma unroll
-            for (int e = 0; e < V; e++) ss = __fmaf_rn(v[i][e], v[i][e], ss);
-        ss = row_sum(ss, T, red[flip]);
+        for (int i = 0; i < C; i++) ss2 = squares(ss2, v[i]);
+        const float ss = row_sum(ss2.x + ss2.y, T, red[flip]);
         flip ^= 1;
         const float ir = 1.0f / sqrtf(ss / (float)a.k + a.eps);
 #pragma unroll
@@ -149,8 +176,7 @@ __global__ void __launch_bounds__(32 * norm_warps(C)) k_fp8_norm(const Fp8ActArg
             const int c = i * T + t;
             const bool in = c < nchunk;
             if (in) Row::store_sum(a, row, c, v[i]);
-#pragma unroll
-            for (int e = 0; e < V; e++) v[i][e] = g[i].e[e] * (v[i][e] * ir);
+            normalise(v[i], g[i].e, ir);
             put<V>(a.o, row, c, v[i], in);
         }
     }
@@ -167,14 +193,14 @@ __global__ void __launch_bounds__(512) k_fp8_norm_long(const Fp8ActArgs a) {
     pdl_wait();
     pdl_launch_dependents();
     Row x;
-    float v[1][V], ss = 0.f;
+    float v[1][V];
+    float2 ss = make_float2(0.f, 0.f);
     for (int c = t; c < nchunk; c += T) {
         x.load(a, row, c, T);
         x.sum(v);
-#pragma unroll
-        for (int e = 0; e < V; e++) ss = __fmaf_rn(v[0][e], v[0][e], ss);
+        ss = squares(ss, v[0]);
     }
-    const float ir = 1.0f / sqrtf(row_sum(ss, T, red) / (float)a.k + a.eps);
+    const float ir = 1.0f / sqrtf(row_sum(ss.x + ss.y, T, red) / (float)a.k + a.eps);
     for (int c0 = 0; c0 < nchunk; c0 += T) {                // whole warps: the lanes of a block stay together
         const int c = c0 + t;
         const bool in = c < nchunk;
@@ -184,8 +210,7 @@ __global__ void __launch_bounds__(512) k_fp8_norm_long(const Fp8ActArgs a) {
         x.load(a, row, c, T);
         x.sum(v);
         if (in) Row::store_sum(a, row, c, v[0]);
-#pragma unroll
-        for (int e = 0; e < V; e++) v[0][e] = g.e[e] * (v[0][e] * ir);
+        normalise(v[0], g.e, ir);
         put<V>(a.o, row, c, v[0], in);
     }
 }
@@ -194,7 +219,7 @@ template <typename TX, typename TR>
 static cudaError_t norm_launch(const Fp8ActArgs &a, cudaStream_t st) {
     constexpr int V = lane_values<TX>(), CMAX = 32 / V;     // at most 32 values of a row a lane
     const int sms = device_sm_count(), warps = (a.k / V + 31) / 32;
-    if (warps > norm_warps(CMAX) * CMAX)
+    if (warps > norm_warps<TX, TR>(CMAX) * CMAX)
         return launch_k(k_fp8_norm_long<TX, TR>, dim3((unsigned)a.n), dim3(512), 0, st, true, a);
     // Chunks a lane and resident warps an SM, as measured (us, 1 / 2 chunks): a few rows are latency, spread over
     // all lanes (1x960 f32 1.6 / 1.9); up to a wave, fewer warps that wait for the row's sum (256x2048 f32 3.2 / 2.7,
@@ -203,7 +228,7 @@ static cudaError_t norm_launch(const Fp8ActArgs &a, cudaStream_t st) {
     const long long rw = (long long)a.n * warps;
     int c = rw <= sms * 4LL || (rw > sms * 32LL && warps <= 8) ? 1 : 2;
     const int resident = c == 1 ? 48 : 32;
-    while (c < CMAX && (warps + c - 1) / c > norm_warps(c)) c <<= 1;
+    while (c < CMAX && (warps + c - 1) / c > norm_warps<TX, TR>(c)) c <<= 1;
     const int w = (warps + c - 1) / c, rows = w == 1 ? 4 : 1;
     const long long ctas = ((long long)a.n - 1) / rows + 1;
     const dim3 grid((unsigned)std::min<long long>(ctas, (long long)sms * std::max(1, resident / (w * rows))));
@@ -218,9 +243,20 @@ static cudaError_t norm_launch(const Fp8ActArgs &a, cudaStream_t st) {
 // Value by value: SwiGLU, and the 8-bit form of x (+ r) as it is
 // ---------------------------------------------------------------------------
 //   SwiGLU: v = x / (1 + exp(-x)) * r;  else h = x + r, r' = rn(h), v = h
-// A thread takes one chunk of a row.  exp and the quotient are the fast forms
-// (each within a few 2^-24 here, against the 2^-4 of the output).  Bound by memory
-// for f32, by instructions for the 16-bit types.
+// A thread takes one chunk of a row.  exp(-x) is the fast 2^t of t = -x log2(e),
+// the quotient the fast reciprocal (each within a few 2^-24, against the 2^-4 of the
+// output); past x = -87 the quotient vanishes.  Bound by memory.
+__device__ __forceinline__ float ex2(float t) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+    return r;
+}
+__device__ __forceinline__ float rcp(float d) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return r;
+}
+
 template <typename TX, typename TR, bool SWIGLU>
 __global__ void __launch_bounds__(256) k_fp8_map(const Fp8ActArgs a) {
     using Row = NormRow<TX, TR, 1>;
@@ -235,9 +271,14 @@ __global__ void __launch_bounds__(256) k_fp8_map(const Fp8ActArgs a) {
     if (in) x.load(a, row, c, 0);
     if constexpr (SWIGLU) {
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float g = fp8_f(x.x[0].e[e]);
-            v[0][e] = in ? __fdividef(g, 1.0f + __expf(-g)) * fp8_f(x.r[0].e[e]) : 0.f;
+        for (int e = 0; e < V; e += 2) {
+            const float2 g = make_float2(fp8_f(x.x[0].e[e]), fp8_f(x.x[0].e[e + 1]));
+            const float2 u = make_float2(fp8_f(x.r[0].e[e]), fp8_f(x.r[0].e[e + 1]));
+            const float2 t = fp8_mul2(g, make_float2(-1.44269504f, -1.44269504f));
+            const float2 d = fp8_add2(make_float2(ex2(t.x), ex2(t.y)), make_float2(1.f, 1.f));
+            const float2 h = fp8_mul2(fp8_mul2(g, make_float2(rcp(d.x), rcp(d.y))), u);
+            v[0][e] = in ? h.x : 0.f;
+            v[0][e + 1] = in ? h.y : 0.f;
         }
     } else {
         x.sum(v);
