@@ -503,6 +503,10 @@ struct Fp8MmtArgs {
     unsigned   *fault;
 };
 
+// Place of 16-byte chunk c of row lr in a half (32 rows x 64 bytes) of a summing
+// warp's way out: the 64-byte swizzle of the TMA store, free of bank conflicts.
+__device__ __forceinline__ int mmt_place(int lr, int c) { return lr * 64 + ((c ^ ((lr >> 1) & 3)) << 4); }
+
 template <int N, typename TY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp8_mm_t(const __grid_constant__ Fp8MmtArgs p) {
     using Cfg = MmtCfg<N>;
@@ -719,7 +723,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
 #pragma unroll
             for (int ps = 0; ps < R / E; ps++) {
                 uint8_t *const stg = out + flip * (32 * 64);
-                auto place = [&](int lr, int c) { return stg + lr * 64 + ((c ^ ((lr >> 1) & 3)) << 4); };
                 flip ^= 1;
                 const int col0 = wrow + ps * E;
                 if (p.vy) {                                               // the copy out of this half, two passes ago
@@ -736,7 +739,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                         v[e] = fp8_t<TY>(lo);
                         v[e + 1] = fp8_t<TY>(hi);
                     }
-                    *reinterpret_cast<uint4 *>(place(lane, c)) = *reinterpret_cast<uint4 *>(v);
+                    *reinterpret_cast<uint4 *>(stg + mmt_place(lane, c)) = *reinterpret_cast<uint4 *>(v);
                 }
                 if (p.vy) {
                     t5_fence_proxy();
@@ -747,13 +750,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                     }
                 } else {
                     __syncwarp();
-                    // rows at any alignment: consecutive lanes write consecutive values
-                    TY *y = static_cast<TY *>(p.a.y);
-                    const int e = lane % E, l0 = lane / E;
-                    if (col0 + e < w.rows)
-#pragma unroll 4
-                        for (int lr = l0; lr < 32 && row0 + lr < p.a.n; lr += 32 / E)
-                            y[(row0 + lr) * p.a.y_ld + col0 + e] = reinterpret_cast<const TY *>(place(lr, e / V))[e % V];
+                    // rows at any alignment: 32 consecutive values of a row an instruction (f32: two passes'), eight
+                    // rows in flight
+                    constexpr int PP = 32 / E;
+                    if (ps % PP == PP - 1) {
+                        const int c0 = col0 - (PP - 1) * E + lane, e = lane % E;
+                        const uint8_t *const src = PP == 1 ? stg : out + (lane / E) * (32 * 64);
+                        const int rows = c0 < w.rows ? (int)min((long long)32, p.a.n - row0) : 0;
+                        TY *y = static_cast<TY *>(p.a.y) + row0 * p.a.y_ld + c0;
+                        for (int b = 0; b < 32; b += 8) {
+                            TY v[8];
+#pragma unroll
+                            for (int u = 0; u < 8; u++)
+                                v[u] = reinterpret_cast<const TY *>(src + mmt_place(b + u, e / V))[e % V];
+#pragma unroll
+                            for (int u = 0; u < 8; u++) {
+                                if (b + u < rows) *y = v[u];
+                                y += p.a.y_ld;
+                            }
+                        }
+                    }
                     __syncwarp();
                 }
             }

@@ -9,9 +9,9 @@ Bounds.  u = 2^-24 is half a step of f32.
    v / s is within DELTA = ((L + 12) / 2 + 10) u of the exact one, and q lies
    between the roundings of v / s (1 - DELTA) and v / s (1 + DELTA).  A scale is
    within DELTA of its own.
- - SwiGLU: exp(-g) is within 2 u (its own error) + 2 u |g| (its argument's, for
+ - SwiGLU: exp(-g) is within 4 u (its own error) + 2 u |g| (its argument's, for
    an exponential formed in base 2) and enters 1 + exp(-g) with weight at most
-   one; the quotient, two products and the scale's add 6 u.  With |g| <= 16 here
+   one; the quotient, two products and the scale's add 8 u.  With |g| <= 16 here
    DELTA = 50 u.
  - A stored residual is off by half a step of its type, and u for the f32 sum.
  - The product: a block's 128 products are exact in f32 and their sum is off by
