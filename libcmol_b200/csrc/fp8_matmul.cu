@@ -36,7 +36,8 @@ struct Fp8MmArgs {
 // the operand of the warp-wide product m16n8k32: the order of k within a block is
 // the same permutation for both operands.  A block's product starts from zero and
 // is scaled and added in f32.  The KW warps of the same rows add up through shared
-// memory, in order.  (tcgen05 takes 128 rows at once, from shared memory: a ring,
+// memory, in order.  4.8 us at 1x2048x11008 (4.7 TB/s), 10.9 at 1x22016x2048 (4.2).
+// (tcgen05 takes 128 rows at once, from shared memory: a ring,
 // 172 CTAs for 22016 rows on 148 SMs and a cluster's sum where rows are few; it
 // measured 11.3 us at 1x22016x2048 and 13.2 us at 1x2048x11008.)
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -152,6 +153,8 @@ __global__ void __launch_bounds__(32 * few_warps(KW), KW > 8 ? 1 : 2) k_fp8_mm_f
 // Barriers, two a block as in k_fp8_mm_t: `full` counts both operands' bytes and
 // the summing warps' release of tensor memory, `done` is the product's commit.
 // Scales come eight blocks at a time.
+//
+// 9.6 us at 37x2048x11008 (eleven blocks a CTA), 17 at 64x22016x2048.
 //
 // Warps: 0 loads, 1 and 2 products in turn (1 also tensor memory), 3 scales, 4-11
 // sums.
@@ -338,6 +341,7 @@ __global__ void __launch_bounds__(MMN_THREADS, 2) k_fp8_mm_n(const __grid_consta
         auto block = [&](auto first, int i) {
             constexpr int F = decltype(first)::value;
             if (i == nb - 1 && p.ksplit > 1) {                             // every product has read its operands
+                __syncwarp();
                 t5_cluster_arrive_all();
                 arrived = true;
             }
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(MMN_THREADS, 2) k_fp8_mm_n(const __grid_consta
                     t5_ld(src + CH * (c + 1), dn);
                 } else {
                     t5_fence_before();
-                    if (lane == 0) mbar_arrive(rel);
+                    t5_arrive(rel, lane == 0);
                     if (i + 1 < nb) {
                         if (!ready) ok = __all_sync(0xffffffffu, wait(&done[st], par, FAULT_GEMV_FULL));
                         t5_fence_after();
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(MMN_THREADS, 2) k_fp8_mm_n(const __grid_consta
             }
             if (i % G == G - 1) {
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sempty[(i / G) & 1]);
+                t5_arrive(&sempty[(i / G) & 1], lane == 0);
             }
         };
         ok = __all_sync(0xffffffffu, wait(&done[0], 0, FAULT_GEMV_FULL));
@@ -472,6 +476,10 @@ __global__ void __launch_bounds__(MMN_THREADS, 2) k_fp8_mm_n(const __grid_consta
 // counts the bytes of both CTAs' stages and the 16 summing warps' release of the
 // part of tensor memory that the block will use, `done` (the products' commit,
 // in both CTAs) frees the stage and hands the sums their block.
+//
+// 354 to 393 us at 8192x22016x2048 from one GPU to another (1.9 to 2.1 PFLOP/s, the
+// tensor pipe half used): the summing warps take ~900 clocks a block of 256 columns,
+// most of it waits for tensor memory one load after another.
 //
 // Warps: 0 loads, 1 and 3 products (rank 0), 2 tensor memory, 4-11 sums.
 #define MMT_SUM_WARPS 8

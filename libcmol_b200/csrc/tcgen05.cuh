@@ -182,6 +182,16 @@ __device__ __forceinline__ void t5_cluster_arrive(uint32_t bar, bool who) {
         : "memory");
 }
 
+// Arrives on a barrier of this CTA from one thread of a warp, without a branch
+// that would part the warp.
+__device__ __forceinline__ void t5_arrive(uint64_t *bar, bool who) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 st;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "@p mbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"((uint32_t)who)
+        : "memory");
+}
+
 // Registers of the calling warpgroup, out of those the block was launched with.
 template <int R>
 __device__ __forceinline__ void t5_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
