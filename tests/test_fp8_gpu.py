@@ -628,3 +628,34 @@ def test_offsets_past_32_bits():
         assert (y[:, :1000] == 0).all()
         del y
     W.free()
+
+
+@pytest.mark.parametrize("n", [1, 5, 12, 40, 130, 700])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_rows_behind_the_last_stay(n, t):
+    """A batch smaller than its buffers: nothing behind row n is written."""
+    from libcmol_b200 import fp8
+    g = _gen(n)
+    rows, k, extra = 384, 768, 130
+    q = torch.full((n + extra, k), 0x2A, dtype=torch.uint8, device="cuda")
+    s = torch.full((6, n + extra), 3.0, device="cuda").t()
+    r = torch.full((n + extra, k), 7.0, dtype=t, device="cuda")
+    r[:n] = _randn(g, n, k, dtype=t)
+    x, w = _randn(g, n, k, dtype=t), torch.ones(k, device="cuda")
+    W = fp8.Fp8Weight.quantize(_weight(g, rows, k))
+    for call in (lambda a, b: fp8.rmsnorm(x, w, 1e-5, residual=r[:n], q=a, scales=b), lambda a, b: fp8.swiglu(x, x, q=a, scales=b),
+                 lambda a, b: fp8.quantize(x, q=a, scales=b)):
+        call(q[:n].view(E4M3), s[:n])
+        assert (q[n:] == 0x2A).all() and (s[n:] == 3).all() and (r[n:] == 7).all()
+    y = torch.full((n + extra, rows), 5.0, dtype=t, device="cuda")
+    W.matmul(q[:n].view(E4M3), s[:n], y=y[:n])
+    assert (y[n:] == 5).all()
+    _mm_check(y[:n], q[:n].view(E4M3), s[:n], *W.read())
+
+
+def test_no_rows():
+    from libcmol_b200 import fp8
+    x = torch.ones(3, 256, device="cuda")[:0]
+    W = fp8.Fp8Weight.quantize(torch.ones(64, 256, device="cuda"))
+    for q, s in (fp8.quantize(x), fp8.swiglu(x, x), fp8.rmsnorm(x, torch.ones(256, device="cuda"), residual=x)):
+        assert q.shape == (0, 256) and s.shape == (0, 2) and W.matmul(q, s).shape == (0, 64)
