@@ -4,9 +4,10 @@
 // A value v of a block is stored as q = rn_e4m3(v / s), s = max(amax / 448,
 // 2^-126), where amax is the block's largest magnitude: 448 is e4m3's largest
 // value, and the floor keeps 1 / s finite for blocks of zeros or of
-// subnormals.  A NaN in a block makes its scale NaN, an infinity makes the
-// scale infinite, and the q of such a block are NaN: every product with it is
-// NaN, as it is NaN or infinite without the rounding to 8 bits.
+// subnormals.  Both quotients are f32's, rounded to nearest.  A NaN in a block
+// makes its scale and its q NaN; an infinity makes the scale infinite, its own q
+// NaN and the finite values' q zero: every product with such a block is NaN, as it
+// is NaN or infinite without the rounding to 8 bits.
 #pragma once
 #include "common.cuh"
 
@@ -159,18 +160,34 @@ __device__ __forceinline__ float fp8_amax(float a, float b, float c) {
     return r;
 }
 
-// Scale of a block from its largest magnitude: within 2^-23 of amax / 448.
-__device__ __forceinline__ float fp8_scale(float amax) {
-    const float s = amax * (1.f / 448.f), lo = 1.17549435e-38f;
-    return s < lo ? lo : s;           // a NaN passes
-}
-
-// 1 / s of a scale (2^-126 <= s <= 2^120, or infinite or NaN, which give NaN):
-// the approximate reciprocal and one Newton step, within 2^-24.
-__device__ __forceinline__ float fp8_inv(float s) {
+// 1 / s of a scale as hi + lo, within 2^-45 of itself: hi is the approximate reciprocal
+// less two units, so below 1 / s, and lo = hi (e + e^2) with the exact e = 1 - s hi.  Then
+// v hi + v lo, with one rounding after the second product, is v / s rounded to nearest
+// (a quotient of f32 values is not that close to a midpoint but once in 2^20 values, and
+// beside e4m3's midpoints, where it would show, far less often); lo >= 0 keeps a zero's
+// sign.  lo is normal up to s = 2^90.
+struct Fp8Inv {
+    float hi, lo;
+};
+#define FP8_MOST_SCALE 1.2379401e27f           // 2^90
+__device__ __forceinline__ Fp8Inv fp8_inv(float s) {
     float r;
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
-    return fmaf(r, fmaf(-s, r, 1.f), r);
+    r *= 0.99999976f;                              // 1 - 2^-22
+    const float e = fmaf(-s, r, 1.f);
+    return {r, r * fmaf(e, e, e)};
+}
+__device__ __forceinline__ float2 fp8_div2(float2 v, Fp8Inv i) {
+    return fp8_fma2(v, make_float2(i.hi, i.hi), fp8_mul2(v, make_float2(i.lo, i.lo)));
+}
+
+// Scale of a block from its largest magnitude: amax / 448 rounded to nearest, after
+// Markstein (1990), by the remainder of a first quotient (exact down to the floor: 448 is
+// 7 * 2^6).
+__device__ __forceinline__ float fp8_scale(float amax) {
+    const float inv = 1.f / 448.f, lo = 1.17549435e-38f, q = amax * inv;
+    const float s = fmaf(fmaf(q, 448.f, -amax), -inv, q);
+    return s < lo ? lo : amax <= 3.40282347e38f ? s : amax;      // infinite and NaN pass
 }
 
 // Two e4m3 values, the first in the low byte (round to nearest even; a NaN
@@ -181,19 +198,29 @@ __device__ __forceinline__ uint32_t fp8_pack2(float lo, float hi) {
     return r;
 }
 
-__device__ __forceinline__ uint2 fp8_pack8(const float v[8], float inv) {
+__device__ __forceinline__ uint2 fp8_pack8(const float *v, Fp8Inv inv) {
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float2 p = fp8_mul2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(inv, inv));
+        const float2 p = fp8_div2(make_float2(v[2 * i], v[2 * i + 1]), inv);
         h[i] = fp8_pack2(p.x, p.y);
     }
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
-// V e4m3 values to consecutive bytes (V-byte aligned).
+// v / s of V values in 8 bits, to consecutive bytes (V-byte aligned).
 template <int V>
-__device__ __forceinline__ void fp8_store(uint8_t *q, const float v[V], float inv) {
+__device__ __forceinline__ void fp8_store(uint8_t *q, float (&v)[V], float s) {
+    Fp8Inv inv = fp8_inv(s);
+    if (s > FP8_MOST_SCALE) {
+        if (s <= 3.40282347e38f) {                 // both 2^-64 times as large: what that loses vanishes in e4m3
+            inv = fp8_inv(s * 5.4210109e-20f);
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] *= 5.4210109e-20f;
+        } else {
+            inv = {0.f, 0.f};                      // infinite: v times zero
+        }
+    }
     if constexpr (V == 8) {
         *reinterpret_cast<uint2 *>(q) = fp8_pack8(v, inv);
     } else {

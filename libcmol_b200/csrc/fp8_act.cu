@@ -36,10 +36,10 @@ struct Fp8ActArgs {
 // Writes V values of (row, chunk c) in 8 bits; the lanes of a block call it
 // together, those past the row with zeros and `in` false.
 template <int V>
-__device__ __forceinline__ void put(const Fp8Out &o, long long row, int c, const float v[V], bool in) {
+__device__ __forceinline__ void put(const Fp8Out &o, long long row, int c, float (&v)[V], bool in) {
     const float s = fp8_scale(fp8_block_amax<V>(v));
     if (!in) return;
-    fp8_store<V>(o.q + row * o.q_ld + (long long)c * V, v, fp8_inv(s));
+    fp8_store<V>(o.q + row * o.q_ld + (long long)c * V, v, s);
     constexpr int L = FP8_BLOCK / V;
     if (c % L == 0) o.s[row * o.s_ld + (long long)(c / L) * o.s_inc] = s;
 }

@@ -61,11 +61,10 @@ __global__ void __launch_bounds__(256) k_fp8_weight_quant(const T *src, long lon
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; i++) amax = fp8_amax(amax, red[i]);
-    const float s = fp8_scale(amax), inv = fp8_inv(s);
+    const float s = fp8_scale(amax);
     uint8_t *t = tiles + ((size_t)rb * w.kblocks + kb) * FP8_TILE_BYTES;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        *reinterpret_cast<uint2 *>(t + fp8_tile_byte(i * 16 + (tid >> 4), c)) = fp8_pack8(v[i], inv);
+    for (int i = 0; i < 8; i++) fp8_store<8>(t + fp8_tile_byte(i * 16 + (tid >> 4), c), v[i], s);
     if (tid == 0) scales[(size_t)rb * w.kblocks + kb] = s;
 }
 
