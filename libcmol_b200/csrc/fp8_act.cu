@@ -137,9 +137,13 @@ __device__ __forceinline__ float row_sum(float v, int T, float *red) {
 }
 
 // Most warps a row: the chunks a lane holds bound the threads that the registers allow.
+// (The 16-bit types without a residual would take 73 registers at 24 warps, which leaves
+// 25 warps an SM where 64 leave 30: 8192x2560 f16 19.5 us against 17.6.)
 template <typename TX, typename TR>
 constexpr int norm_warps(int c) {
-    return c == 1 ? 24 : c == 2 && !(sizeof(TX) == 2 && std::is_same<TR, float>::value) ? 16 : 12;
+    constexpr bool half = sizeof(TX) == 2;
+    return c == 1 ? (half && std::is_same<TR, Fp8None>::value ? 32 : 24)
+                  : c == 2 && !(half && std::is_same<TR, float>::value) ? 16 : 12;
 }
 
 template <typename TX, typename TR, int C>

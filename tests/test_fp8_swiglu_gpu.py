@@ -1,11 +1,13 @@
 """SwiGLU's value before its rounding to 8 bits, read from the scales: with one
 gate that is not zero in a block, the block's scale is |v| / 448 in f32.
 
-Bound, u = 2^-24.  exp is within 2 units of its last place (4 u), the sum with
-one, the quotient, the product with up and the scale's quotient u each: 8 u.
-Where exp(-gate) overflows, v = gate * exp(gate/2) * up * exp(gate/2): two
-exponentials (8 u), three products and the scale's quotient: 12 u.  Terms of second order
-are far below one more u: 13 u for both."""
+Bound, u = 2^-24.  Up to |gate| = 87: the power of two is within 2 units of its
+last place (4 u), 1 + exp(-gate) takes two roundings (2 u), the reciprocal is within
+one unit (2 u), the two products and the scale's quotient u each: 11 u, and 87 times the
+error of f32's ln(2) in the exponent, 2.8e-9: 4.1 u.
+Below -87, v = gate * exp(gate/2) * up * exp(gate/2): two exponentials (2 units, 4 u each), three
+products and the scale's quotient: 12 u.  Terms of second order are far below one more u:
+16 u for both."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -37,7 +39,7 @@ def _one_a_block(g, u, where):
     return gate, up
 
 
-@pytest.mark.parametrize("lo, hi", [(-16, 16), (-30, -16), (-60, -30), (-80, -60), (-88.7, -80), (-104, -88), (-174, -104),
+@pytest.mark.parametrize("lo, hi", [(-16, 16), (-30, -16), (-60, -30), (-80, -60), (-88.7, -80), (-104, -88), (-170, -104), (86, 88),
                                     (16, 1000)])
 @pytest.mark.parametrize("t", [F32, BF16])
 def test_accuracy(lo, hi, t):
@@ -53,28 +55,49 @@ def test_accuracy(lo, hi, t):
     keep = want.abs() >= 448 * LOWEST
     assert keep.any()
     err = (s[:, 0].double() * 448 - want.abs()).abs()[keep]
-    assert (err <= 13 * U * want.abs()[keep]).all(), (err / want.abs()[keep]).max().item() / U
+    assert (err <= 16 * U * want.abs()[keep]).all(), (err / want.abs()[keep]).max().item() / U
     top = q[torch.arange(n, device="cuda"), where].double()[keep]
     assert (top == 448 * want[keep].sign()).all()
     assert (s[:, 1] == LOWEST).all()
 
 
-def test_a_value_does_not_depend_on_its_neighbours():
-    """Gates far out, infinite or NaN in one block leave the bits of the others as they are."""
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_a_value_does_not_depend_on_its_neighbours(t):
+    """Gates far out beside an ordinary one, whose value sets the scale, leave its bits as they are."""
     from libcmol_b200 import fp8
+    n = 4096
     r = torch.Generator(device="cuda").manual_seed(7)
-    n, k = 64, 1024
-    gate = 20 * torch.randn(n, k, generator=r, device="cuda")
-    up = torch.randn(n, k, generator=r, device="cuda")
+    g = (3 * torch.randn(n, generator=r, device="cuda")).to(t)
+    u = (1 + torch.rand(n, generator=r, device="cuda")).to(t)
+    where = 32 + torch.randint(0, 64, (n,), generator=r, device="cuda")
+    gate, up = _one_a_block(g, u, where)
     q0, s0 = fp8.swiglu(gate, up)
-    far = gate.clone()
-    far[:, 256:264] = torch.tensor([-89.0, -1e4, -float("inf"), float("inf"), float("nan"), -120.0, -3e38, 3e38], device="cuda")
-    q1, s1 = fp8.swiglu(far, up)
-    keep = [b for b in range(8) if b != 2]
-    assert torch.equal(s0[:, keep], s1[:, keep])
-    a, b = (q.view(torch.uint8).view(n, 8, 128)[:, keep] for q in (q0, q1))
-    assert torch.equal(a, b)
-    assert torch.isnan(s1[:, 2]).all()
+    for far in (-86.9, -87.1, -88.5, -89.0, -200.0, -3e38):
+        for col in (0, 31, 96, 127, 130):
+            other = gate.clone()
+            other[:, col] = far
+            q1, s1 = fp8.swiglu(other, up)
+            assert torch.equal(s0[:, 0], s1[:, 0])
+            keep = q0.view(torch.uint8)[:, :128] == q1.view(torch.uint8)[:, :128]
+            if col < 128:
+                keep[:, col] = True
+            assert keep.all()
+
+
+def test_nan_and_infinite_gates_stay_in_their_block():
+    from libcmol_b200 import fp8
+    r = torch.Generator(device="cuda").manual_seed(8)
+    gate, up = 3 * torch.randn(64, 1024, generator=r, device="cuda"), torch.randn(64, 1024, generator=r, device="cuda")
+    q0, s0 = fp8.swiglu(gate, up)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        far = gate.clone()
+        far[:, 300] = bad
+        q1, s1 = fp8.swiglu(far, up)
+        keep = [b for b in range(8) if b != 2]
+        assert torch.equal(s0[:, keep], s1[:, keep])
+        a, b = (q.view(torch.uint8).view(64, 8, 128)[:, keep] for q in (q0, q1))
+        assert torch.equal(a, b)
+        assert torch.isinf(s1[:, 2]).all() if bad == float("inf") else torch.isnan(s1[:, 2]).all()
 
 
 def test_infinite_gates():
