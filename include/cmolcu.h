@@ -173,7 +173,8 @@ int cmolcu_fp8_rmsnorm(int device, const void *x, int x_dtype, long long x_ld,
                        const float *norm_w, float eps, int n, int k,
                        void *q, long long q_ld, float *scales, long long s_ld, long long s_inc, void *stream);
 
-/* v = gate / (1 + exp(-gate)) * up; q and scales of v.  gate and up are rows
+/* v = gate / (1 + exp(-gate)) * up, within 2^-20 of itself in f32 (also where
+ * exp(-gate) overflows); q and scales of v.  gate and up are rows
  * of k values of `dtype`; both may be parts of one buffer (the product of the
  * stacked gate and up weights: up = gate + k, both strides 2 k). */
 int cmolcu_fp8_swiglu(int device, const void *gate, long long gate_ld, const void *up, long long up_ld, int dtype,

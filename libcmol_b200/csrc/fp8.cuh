@@ -229,12 +229,14 @@ __device__ __forceinline__ void fp8_store(uint8_t *q, float (&v)[V], float s) {
     }
 }
 
-// Largest magnitude of the 128 values that 128 / V consecutive lanes hold, V each.
+// Largest magnitude of the 128 values that 128 / V consecutive lanes hold, V each;
+// lanes that are not `in` count as zeros.
 template <int V>
-__device__ __forceinline__ float fp8_block_amax(const float v[V]) {
+__device__ __forceinline__ float fp8_block_amax(const float v[V], bool in) {
     float a = 0.f;
 #pragma unroll
     for (int i = 0; i < V; i += 2) a = fp8_amax(a, v[i], v[i + 1]);
+    a = in ? a : 0.f;
 #pragma unroll
     for (int o = FP8_BLOCK / V / 2; o > 0; o >>= 1) a = fp8_amax(a, __shfl_xor_sync(0xffffffffu, a, o));
     return a;

@@ -34,10 +34,10 @@ struct Fp8ActArgs {
 };
 
 // Writes V values of (row, chunk c) in 8 bits; the lanes of a block call it
-// together, those past the row with zeros and `in` false.
+// together, those past the row with `in` false.
 template <int V>
 __device__ __forceinline__ void put(const Fp8Out &o, long long row, int c, float (&v)[V], bool in) {
-    const float s = fp8_scale(fp8_block_amax<V>(v));
+    const float s = fp8_scale(fp8_block_amax<V>(v, in));
     if (!in) return;
     fp8_store<V>(o.q + row * o.q_ld + (long long)c * V, v, s);
     constexpr int L = FP8_BLOCK / V;
@@ -247,10 +247,13 @@ static cudaError_t norm_launch(const Fp8ActArgs &a, cudaStream_t st) {
 // Value by value: SwiGLU, and the 8-bit form of x (+ r) as it is
 // ---------------------------------------------------------------------------
 //   SwiGLU: v = x / (1 + exp(-x)) * r;  else h = x + r, r' = rn(h), v = h
-// A thread takes one chunk of a row.  exp(-x) is the fast 2^t of t = -x log2(e),
-// the quotient the fast reciprocal (each within a few 2^-24, against the 2^-4 of the
-// output); past x = -87 the quotient vanishes.  Bound by memory: 68 us at 8192x11008 bf16
-// (6.6 TB/s), the 8-bit form alone 22.2 at 4099x11008 f16 (6.2).
+// A thread takes one chunk of a row.  Bound by memory: 71 us at 8192x11008 bf16
+// (6.4 TB/s), the 8-bit form alone 22.4 at 4099x11008 f16 (6.1).
+//
+// SwiGLU in f32, within 16 * 2^-24 before the 8 bits: exp(-x) = 2^t (1 - n) is the fast 2^t
+// of the rounded t = -x log2(e) with n = x + t ln(2) to first order (t's rounding alone
+// would cost |x| 2^-24; n^2 is below 2^-33, and f32's ln(2) is off by 2^-28 of itself),
+// and the quotient the fast reciprocal.  Each is within two units of the last place.
 __device__ __forceinline__ float ex2(float t) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
@@ -260,6 +263,21 @@ __device__ __forceinline__ float rcp(float d) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
     return r;
+}
+__device__ __forceinline__ float2 swiglu2(float2 x, float2 r) {
+    const float c = -1.44269502f, l = 0.693147182f;
+    const float2 t = fp8_mul2(x, make_float2(c, c)), m = make_float2(-1.f, -1.f);
+    const float2 n = fp8_fma2(t, make_float2(l, l), x);
+    const float2 h = make_float2(ex2(t.x), ex2(t.y));
+    const float2 d = fp8_fma2(h, n, fp8_fma2(h, m, m));                          // -(1 + exp(-x))
+    return fp8_mul2(fp8_mul2(x, make_float2(rcp(-d.x), rcp(-d.y))), r);
+}
+// Past |x| = 87, where exp(-x) or the reciprocal leaves f32's normal numbers: x exp(x/2) r exp(x/2),
+// which may lie far above the scales' floor (x = -100 with r = 2^120 gives -5e-6).
+__device__ __forceinline__ float swiglu_far(float x, float r) {
+    if (x > 0.f) return x * r;
+    const float p = expf(0.5f * x);
+    return x * p * r * p;
 }
 
 template <typename TX, typename TR, bool SWIGLU>
@@ -275,21 +293,27 @@ __global__ void __launch_bounds__(256) k_fp8_map(const Fp8ActArgs a) {
     Row x;
     if (in) x.load(a, row, c, 0);
     if constexpr (SWIGLU) {
+        float most = 0.f;
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
             const float2 g = make_float2(fp8_f(x.x[0].e[e]), fp8_f(x.x[0].e[e + 1]));
-            const float2 u = make_float2(fp8_f(x.r[0].e[e]), fp8_f(x.r[0].e[e + 1]));
-            const float2 t = fp8_mul2(g, make_float2(-1.44269504f, -1.44269504f));
-            const float2 d = fp8_add2(make_float2(ex2(t.x), ex2(t.y)), make_float2(1.f, 1.f));
-            const float2 h = fp8_mul2(fp8_mul2(g, make_float2(rcp(d.x), rcp(d.y))), u);
-            v[0][e] = in ? h.x : 0.f;
-            v[0][e + 1] = in ? h.y : 0.f;
+            most = fp8_amax(most, g.x, g.y);
+            const float2 h = swiglu2(g, make_float2(fp8_f(x.r[0].e[e]), fp8_f(x.r[0].e[e + 1])));
+            v[0][e] = h.x;
+            v[0][e + 1] = h.y;
+        }
+        if (in && !(most <= 87.f)) {                        // read again: kept, they would cost registers
+            const TX *gate = static_cast<const TX *>(a.x) + row * a.x_ld + (long long)c * V;
+            const TR *up = static_cast<const TR *>(a.r) + row * a.r_ld + (long long)c * V;
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float g = fp8_f(gate[e]);
+                if (fabsf(g) > 87.f) v[0][e] = swiglu_far(g, fp8_f(up[e]));
+            }
         }
     } else {
         x.sum(v);
         if (in) Row::store_sum(a, row, c, v[0]);
-#pragma unroll
-        for (int e = 0; e < V; e++) v[0][e] = in ? v[0][e] : 0.f;
     }
     put<V>(a.o, row, c, v[0], in);
 }
