@@ -58,7 +58,7 @@ struct Fp8Device {
         }                                                                       \
     } while (0)
 
-// Device fault word of the kernels behind cmolcu.h (seam.cu).
+// Device fault word of the kernels behind cmolcu.h (seam.cu), null where there is none.
 unsigned int *cmolcu_fault_word(int device);
 
 // ---------------------------------------------------------------------------

@@ -1,5 +1,6 @@
 // seam.cu — the C ABI of cmolcu.h (weights, GEMV, host matmul seam).
 #include "../../include/cmolcu.h"
+#include "fp8.cuh"
 #include "gemm_tc.cuh"
 #include "gemv_launch.cuh"
 
@@ -7,6 +8,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 #include <string>
 
 static thread_local char g_err[512];
@@ -21,26 +24,35 @@ extern "C" void cmolcu_set_error(const char *fmt, ...) {
 extern "C" const char *cmolcu_last_error(void) { return g_err; }
 
 // One fault word per device for kernels launched through this seam.
-static unsigned int *g_fault[64];
+static std::atomic<unsigned int *> g_fault[64];
 
 unsigned int *cmolcu_fault_word(int device) {
     if (device < 0 || device >= 64) return nullptr;
-    if (!g_fault[device]) {
-        unsigned int *p = nullptr;
-        if (cudaMalloc(&p, sizeof(unsigned int)) != cudaSuccess) return nullptr;
-        cudaMemset(p, 0, sizeof(unsigned int));
-        g_fault[device] = p;
+    unsigned int *p = g_fault[device];
+    if (p) return p;
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lock(mu);
+    if ((p = g_fault[device])) return p;
+    Fp8Device dev(device);                                 // the word lies on the device whose kernels write it
+    cudaError_t e = dev.err;
+    if (e == cudaSuccess) e = cudaMalloc(&p, sizeof(unsigned int));
+    if (e == cudaSuccess) e = cudaMemset(p, 0, sizeof(unsigned int));
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
     }
-    return g_fault[device];
+    return g_fault[device] = p;
 }
 
 extern "C" int cmolcu_fault_status(int device, unsigned int *code, int clear) {
+    static const char *who = "cmolcu_fault_status";
     unsigned int *p = cmolcu_fault_word(device);
-    if (!p) { cmolcu_set_error("no fault word for device %d", device); return -1; }
+    if (!p) { cmolcu_set_error("%s: no fault word for device %d", who, device); return -1; }
     unsigned int v = 0;
-    CUDA_TRY(cudaSetDevice(device));
-    CUDA_TRY(cudaMemcpy(&v, p, sizeof v, cudaMemcpyDeviceToHost));
-    if (clear && v) CUDA_TRY(cudaMemset(p, 0, sizeof(unsigned int)));
+    Fp8Device dev(device);
+    FP8_TRY(who, dev.err);
+    FP8_TRY(who, cudaMemcpy(&v, p, sizeof v, cudaMemcpyDeviceToHost));
+    if (clear && v) FP8_TRY(who, cudaMemset(p, 0, sizeof(unsigned int)));
     if (code) *code = v;
     return 0;
 }
