@@ -206,7 +206,8 @@ size_t cmolcu_fp8_weight_bytes(const cmolcu_fp8_weight_t *w);   /* values and sc
 /* y(c, r) = sum_b sx(c, b) * sw(r/128, b) * sum_{k in b} qx(c, k) * qw(r, k) for
  * n >= 1 activation rows: y is [n][rows] of y_dtype (CMOLCU_F32, _F16 or
  * _BF16), y_ld values apart.  Products and sums in f32, one rounding at the
- * end.  Waits inside the kernels are bounded (cmolcu_fault_status). */
+ * end.  Waits inside the kernels are bounded: where one runs out y is invalid and the
+ * device's fault word says so once the kernel has finished (cmolcu_fault_status). */
 int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
                       const float *scales, long long s_ld, long long s_inc, int n,
                       void *y, int y_dtype, long long y_ld, void *stream);

@@ -13,7 +13,8 @@ layer, for instance::
 Every call launches on torch's current stream of the tensors' device and can
 be captured in a CUDA graph (making a weight cannot).  Results go to the
 tensors given, or to new ones.  k is a multiple of 16; the rows of a `q` start
-on 16-byte boundaries.
+on 16-byte boundaries.  Waits inside the products are bounded: `fault` tells whether
+one ran out.
 """
 
 from __future__ import annotations
@@ -124,6 +125,16 @@ def rmsnorm(x, norm_w, eps: float = 1e-5, residual=None, residual_out=None, q=No
                                 eps, n, k, q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, _stream(index)):
         check(-1, "fp8.rmsnorm")
     return q, scales
+
+
+def fault(device: int = 0, clear: bool = False) -> int:
+    """The fault word of this module's products on a GPU: 0, or the code of a
+    bounded wait inside a kernel that ran out (cmolcu_fault_status); the products
+    since the last look are then invalid.  It counts what has finished: synchronize
+    first.  `clear` resets it."""
+    code = C.c_uint(0)
+    check(lib().cmolcu_fault_status(device, C.byref(code), int(clear)), "fp8.fault")
+    return code.value
 
 
 def quantize(x, q=None, scales=None):
