@@ -190,7 +190,9 @@ int cmolcu_fp8_swiglu(int device, const void *gate, long long gate_ld, const voi
  *                   to device memory on `stream`
  * The three that make a weight allocate and wait for `stream`; they cannot be
  * captured.  A weight can be used by any number of streams and threads at
- * once.  Free it when no product that reads it is left to run. */
+ * once.  Free it when no product that reads it is left to run: a graph with a
+ * captured product holds the weight's memory by address and does not keep it alive.
+ * Freeing waits for the device and is allowed while a stream is captured. */
 typedef struct cmolcu_fp8_weight cmolcu_fp8_weight_t;
 int    cmolcu_fp8_weight_upload(int device, const void *q, const float *scales, int rows, int k,
                                 cmolcu_fp8_weight_t **out);

@@ -203,7 +203,12 @@ extern "C" int cmolcu_fp8_weight_read_dev(const cmolcu_fp8_weight_t *h, void *q,
 extern "C" void cmolcu_fp8_weight_free(cmolcu_fp8_weight_t *h) {
     if (!h) return;
     Fp8Device dev(h->device);
-    cudaFree(h->base);
+    // A handle may go, collected in some language's runtime, while a stream is captured, by this thread or another:
+    // only in the relaxed mode does freeing memory leave that capture alone.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (cudaFree(h->base) != cudaSuccess) cudaGetLastError();
+    if (e == cudaSuccess) cudaThreadExchangeStreamCaptureMode(&mode);
     delete h;
 }
 

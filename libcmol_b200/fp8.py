@@ -162,7 +162,11 @@ class Fp8Weight:
     [ceil(rows/128), ceil(k/128)] float32, both on a GPU, or both on the host
     (then `device` says where the weight goes).
     Fp8Weight.quantize(w): from a float32, float16 or bfloat16 matrix on a
-    GPU."""
+    GPU.
+
+    The memory goes with the last reference (or with `free`), which may be while a
+    stream is captured.  A CUDA graph with a captured product does not keep the
+    weight: hold on to it as long as the graph is replayed."""
 
     def __init__(self, q, scales, device: int = 0):
         what = "Fp8Weight"
