@@ -15,6 +15,10 @@ be captured in a CUDA graph (making a weight cannot).  Results go to the
 tensors given, or to new ones.  k is a multiple of 16; the rows of a `q` start
 on 16-byte boundaries.  Waits inside the products are bounded: `fault` tells whether
 one ran out.
+
+The operators are for inference: they have no backward pass, and activations that
+require a gradient are refused while gradients are recorded.  Gains and weights may be
+parameters and count as constants.
 """
 
 from __future__ import annotations
@@ -68,6 +72,13 @@ def _first(t, what: str, dtypes):
     return index, shape, _rows(t, what, dtypes, shape, index)
 
 
+def _no_grad(what: str, **tensors):
+    """Refuses activations that autograd follows: their results would be cut off without a word."""
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise CmolError(f"{what}: {name} requires a gradient and there is none here: call it under torch.no_grad()")
+
+
 def _scales(t, what: str, shape, index: int):
     if t.shape != shape or t.dtype is not torch.float32 or t.get_device() != index:
         raise CmolError(f"{what}: scales are float32 {shape} on cuda:{index}, got {t.dtype} {tuple(t.shape)} on "
@@ -102,6 +113,8 @@ def rmsnorm(x, norm_w, eps: float = 1e-5, residual=None, residual_out=None, q=No
     itself when not given); q, scales of norm_w * h / sqrt(mean(h^2) + eps), or
     of h itself when norm_w is None.  x and residual are [n, k] float32,
     float16 or bfloat16, norm_w is [k] float32."""
+    if torch.is_grad_enabled():
+        _no_grad("fp8.rmsnorm", x=x, residual=residual, residual_out=residual_out, scales=scales)
     index, shape, x_ld = _first(x, "fp8.rmsnorm: x", _TAG)
     n, k = shape
     q, q_ld, scales, s_ld, s_inc = _out(q, scales, "fp8.rmsnorm: q", shape, index)
@@ -145,6 +158,8 @@ def quantize(x, q=None, scales=None):
 def swiglu(gate, up, q=None, scales=None):
     """q, scales of gate / (1 + exp(-gate)) * up; gate and up [n, k] of one
     type, which may be halves of one tensor."""
+    if torch.is_grad_enabled():
+        _no_grad("fp8.swiglu", gate=gate, up=up, scales=scales)
     index, shape, g_ld = _first(gate, "fp8.swiglu: gate", _TAG)
     u_ld = _rows(up, "fp8.swiglu: up", (gate.dtype,), shape, index)
     q, q_ld, scales, s_ld, s_inc = _out(q, scales, "fp8.swiglu: q", shape, index)
@@ -220,6 +235,8 @@ class Fp8Weight:
     def matmul(self, q, scales, y=None, dtype=torch.float32):
         """y [n, rows] = (q * scales) . W^T in float32, float16 or bfloat16
         (`y`'s type, else `dtype`)."""
+        if torch.is_grad_enabled():
+            _no_grad("Fp8Weight.matmul", scales=scales, y=y)
         index = self.index
         n = q.shape[0]
         q_ld = _rows(q, "Fp8Weight.matmul: q", _Q, (n, self.k), index)

@@ -3,6 +3,7 @@ stand-in for the library where a call would need a GPU."""
 import ctypes as C
 
 import pytest
+import torch
 
 import libcmol_b200 as pkg
 from libcmol_b200 import fp8
@@ -33,3 +34,33 @@ def test_a_wait_that_ran_out_is_seen(monkeypatch):
 def test_no_word_is_an_error():
     with pytest.raises(pkg.CmolError, match="fp8.fault: cmolcu_fault_status: no fault word for device 99"):
         fp8.fault(99)
+
+
+def test_activations_that_require_a_gradient_are_refused():
+    """While gradients are recorded; the results would be cut from the graph without a word."""
+    g, x = torch.zeros(2, 256, requires_grad=True), torch.zeros(2, 256)
+    s = torch.zeros(2, 2, requires_grad=True)
+    W = fp8.Fp8Weight.__new__(fp8.Fp8Weight)
+    W.h, W.rows, W.k, W.index = None, 2, 256, 0
+    q = x.to(torch.float8_e4m3fn)
+    gains = torch.nn.Parameter(torch.ones(256))
+    for call, name in [
+        (lambda: fp8.rmsnorm(g, gains), "fp8.rmsnorm: x"),
+        (lambda: fp8.rmsnorm(x, gains, residual=g), "fp8.rmsnorm: residual"),
+        (lambda: fp8.rmsnorm(x, gains, residual=x, residual_out=g), "fp8.rmsnorm: residual_out"),
+        (lambda: fp8.rmsnorm(x, gains, scales=s), "fp8.rmsnorm: scales"),
+        (lambda: fp8.quantize(g), "fp8.rmsnorm: x"),
+        (lambda: fp8.swiglu(g, x), "fp8.swiglu: gate"),
+        (lambda: fp8.swiglu(x, g), "fp8.swiglu: up"),
+        (lambda: W.matmul(q, s), "Fp8Weight.matmul: scales"),
+        (lambda: W.matmul(q, x[:, :2], y=g), "Fp8Weight.matmul: y"),
+    ]:
+        with pytest.raises(pkg.CmolError) as e:
+            call()
+        assert str(e.value).startswith(name + " requires a gradient"), str(e.value)
+        with torch.no_grad(), pytest.raises(pkg.CmolError, match="on cpu|shape|scales are"):
+            call()
+    with pytest.raises(pkg.CmolError, match="wanted a GPU"):         # gains may be a parameter
+        fp8.rmsnorm(x, gains)
+    with pytest.raises(pkg.CmolError, match="wanted a GPU"):         # and so may a weight that is quantised
+        fp8.Fp8Weight.quantize(torch.nn.Parameter(torch.zeros(2, 256)))
