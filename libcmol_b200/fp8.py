@@ -75,7 +75,7 @@ def _first(t, what: str, dtypes):
 def _no_grad(what: str, **tensors):
     """Refuses activations that autograd follows: their results would be cut off without a word."""
     for name, t in tensors.items():
-        if t is not None and t.requires_grad:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise CmolError(f"{what}: {name} requires a gradient and there is none here: call it under torch.no_grad()")
 
 
@@ -104,6 +104,9 @@ def _stream(index: int) -> int:
 
 # The same without building a stream object (2 us a call), where torch offers it.
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
+# Counts tensors as modified, so that a backward pass which saved one does not take it for
+# what it was (the public form checks its argument first, 0.2 us a call).
+_modified = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)
 
 
 def rmsnorm(x, norm_w, eps: float = 1e-5, residual=None, residual_out=None, q=None, scales=None):
@@ -113,7 +116,8 @@ def rmsnorm(x, norm_w, eps: float = 1e-5, residual=None, residual_out=None, q=No
     itself when not given); q, scales of norm_w * h / sqrt(mean(h^2) + eps), or
     of h itself when norm_w is None.  x and residual are [n, k] float32,
     float16 or bfloat16, norm_w is [k] float32."""
-    if torch.is_grad_enabled():
+    if x.requires_grad or (residual is not None and residual.requires_grad) or (
+            residual_out is not None and residual_out.requires_grad) or (scales is not None and scales.requires_grad):
         _no_grad("fp8.rmsnorm", x=x, residual=residual, residual_out=residual_out, scales=scales)
     index, shape, x_ld = _first(x, "fp8.rmsnorm: x", _TAG)
     n, k = shape
@@ -137,6 +141,7 @@ def rmsnorm(x, norm_w, eps: float = 1e-5, residual=None, residual_out=None, q=No
     if lib().cmolcu_fp8_rmsnorm(index, x.data_ptr(), _TAG[x.dtype], x_ld, r_ptr, r_ld, ro_ptr, ro_ld, r_tag, w_ptr,
                                 eps, n, k, q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, _stream(index)):
         check(-1, "fp8.rmsnorm")
+    _modified([scales] if residual is None else [scales, residual if residual_out is None else residual_out])
     return q, scales
 
 
@@ -158,7 +163,7 @@ def quantize(x, q=None, scales=None):
 def swiglu(gate, up, q=None, scales=None):
     """q, scales of gate / (1 + exp(-gate)) * up; gate and up [n, k] of one
     type, which may be halves of one tensor."""
-    if torch.is_grad_enabled():
+    if gate.requires_grad or up.requires_grad or (scales is not None and scales.requires_grad):
         _no_grad("fp8.swiglu", gate=gate, up=up, scales=scales)
     index, shape, g_ld = _first(gate, "fp8.swiglu: gate", _TAG)
     u_ld = _rows(up, "fp8.swiglu: up", (gate.dtype,), shape, index)
@@ -167,6 +172,7 @@ def swiglu(gate, up, q=None, scales=None):
     if lib().cmolcu_fp8_swiglu(index, gate.data_ptr(), g_ld, up.data_ptr(), u_ld, _TAG[gate.dtype], n, k,
                                q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, _stream(index)):
         check(-1, "fp8.swiglu")
+    _modified([scales])
     return q, scales
 
 
@@ -235,7 +241,7 @@ class Fp8Weight:
     def matmul(self, q, scales, y=None, dtype=torch.float32):
         """y [n, rows] = (q * scales) . W^T in float32, float16 or bfloat16
         (`y`'s type, else `dtype`)."""
-        if torch.is_grad_enabled():
+        if scales.requires_grad or (y is not None and y.requires_grad):
             _no_grad("Fp8Weight.matmul", scales=scales, y=y)
         index = self.index
         n = q.shape[0]
@@ -247,6 +253,7 @@ class Fp8Weight:
         if lib().cmolcu_fp8_matmul(self.h, q.data_ptr(), q_ld, scales.data_ptr(), s_ld, s_inc, n, y.data_ptr(),
                                    _TAG[y.dtype], y_ld, _stream(index)):
             check(-1, "Fp8Weight.matmul")
+        _modified([y])
         return y
 
     def free(self):
