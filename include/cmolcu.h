@@ -214,6 +214,21 @@ int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_l
                       const float *scales, long long s_ld, long long s_inc, int n,
                       void *y, int y_dtype, long long y_ld, void *stream);
 
+/* The product has several forms, which differ in which operand's rows are the tensor
+ * core's M and in their tiles:
+ *   CMOLCU_FP8_FEW  up to 16 rows, from memory to registers;
+ *   16, 32, 64      that many activation rows by 128 weight rows a CTA, k split over a
+ *                   cluster where CTAs are few;
+ *   128, 256        256 activation rows by that many weight rows a pair of CTAs.
+ * _form says which one a call with n rows takes (0: n < 1 or no weight); _as runs a given one
+ * (_FEW up to 16 rows, the others any n).  For tests and measurements: sums are split
+ * differently, so last bits differ. */
+#define CMOLCU_FP8_FEW 8
+int cmolcu_fp8_matmul_form(const cmolcu_fp8_weight_t *w, int n);
+int cmolcu_fp8_matmul_as(int form, const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
+                         const float *scales, long long s_ld, long long s_inc, int n,
+                         void *y, int y_dtype, long long y_ld, void *stream);
+
 /* ---- host-only tokenizer -------------------------------------------------
  * The vocabulary of a GGUF file without loading weights or using a GPU:
  * the same encoder and decoder cmol_encode / cmol_decode_token use

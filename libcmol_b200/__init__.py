@@ -86,6 +86,8 @@ def _declare(L):
     sig("cmolcu_fp8_weight_free", None, [_vp])
     sig("cmolcu_fp8_weight_bytes", C.c_size_t, [_vp])
     sig("cmolcu_fp8_matmul", C.c_int, [_vp, _vp, ll, _vp, ll, ll, C.c_int, _vp, C.c_int, ll, _vp])
+    sig("cmolcu_fp8_matmul_form", C.c_int, [_vp, C.c_int])
+    sig("cmolcu_fp8_matmul_as", C.c_int, [C.c_int, _vp, _vp, ll, _vp, ll, ll, C.c_int, _vp, C.c_int, ll, _vp])
     for name, res, args in _EXTRA_SIGS:
         if hasattr(L, name):
             sig(name, res, args)

@@ -976,10 +976,8 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
 // 4.1, 8x22016x2048 11.5 against 10.7), beyond while the matrix is small, as it reads
 // the activations again for every 16 weight rows (16x5760x960 3.8 against 4.2,
 // 16x11008x2048 8.5 against 6.5).
-template <typename TY>
-static cudaError_t mm_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
-    if (a.n <= 8) return few_launch<1, TY>(a, st);
-    if (a.n <= 16 && (long long)a.w.rows * a.w.k < 12 << 20) return few_launch<2, TY>(a, st);
+static int mm_form(const Fp8MmArgs &a) {
+    if (a.n <= 8 || (a.n <= 16 && (long long)a.w.rows * a.w.k < 12 << 20)) return CMOLCU_FP8_FEW;
     const int sms = device_sm_count(), nts[3] = {16, 32, 64};
     const double per[3] = {0.40, 0.50, 0.80};
     double best = 1e30;
@@ -996,7 +994,13 @@ static cudaError_t mm_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st)
         const double t = 3.3 + rounds * (n == 128 ? a.w.kblocks * 0.25 + 0.5 : a.w.kblocks * 0.47 + 1.5);
         if (t < best) { best = t; form = n; }
     }
+    return form;
+}
+
+template <typename TY>
+static cudaError_t mm_run(int form, const Fp8MmArgs &a, unsigned *fault, cudaStream_t st) {
     switch (form) {
+    case CMOLCU_FP8_FEW: return a.n <= 8 ? few_launch<1, TY>(a, st) : few_launch<2, TY>(a, st);
     case 16: return mmn_launch<16, TY>(a, fault, st);
     case 32: return mmn_launch<32, TY>(a, fault, st);
     case 64: return mmn_launch<64, TY>(a, fault, st);
@@ -1005,21 +1009,23 @@ static cudaError_t mm_pick(const Fp8MmArgs &a, unsigned *fault, cudaStream_t st)
     }
 }
 
-extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld, const float *scales,
-                                 long long s_ld, long long s_inc, int n, void *y, int y_dtype, long long y_ld,
-                                 void *stream) {
-    static const char *who = "cmolcu_fp8_matmul";
+static int matmul(const char *who, int form, const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
+                  const float *scales, long long s_ld, long long s_inc, int n, void *y, int y_dtype, long long y_ld,
+                  void *stream) {
     if (!w) { cmolcu_set_error("%s: NULL argument", who); return -1; }
     if (n < 0 || n > 1 << 30) { cmolcu_set_error("%s: n=%d", who, n); return -1; }
     if (!fp8_elem_bytes(y_dtype)) { cmolcu_set_error("%s: unsupported dtype %d", who, y_dtype); return -1; }
     if (n == 0) return 0;
     if (!q || !scales || !y) { cmolcu_set_error("%s: NULL argument", who); return -1; }
-    if (n == 1) q_ld = (w->w.k + 15) / 16 * 16;        // a single row has no stride
+    if (n == 1) {                                       // a single row has no stride
+        q_ld = (w->w.k + 15) / 16 * 16;
+        y_ld = (w->w.rows + 15LL) / 16 * 16;
+    }
     if ((reinterpret_cast<uintptr_t>(q) & 15) || q_ld < w->w.k || q_ld % 16) {
         cmolcu_set_error("%s: q rows must start on 16-byte boundaries (q_ld=%lld)", who, q_ld);
         return -1;
     }
-    if (n > 1 && y_ld < w->w.rows) { cmolcu_set_error("%s: rows of y overlap (y_ld=%lld)", who, y_ld); return -1; }
+    if (y_ld < w->w.rows) { cmolcu_set_error("%s: rows of y overlap (y_ld=%lld)", who, y_ld); return -1; }
     Fp8Device dev(w->device);
     FP8_TRY(who, dev.err);
     Fp8MmArgs a = {};
@@ -1027,10 +1033,38 @@ extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, lo
     a.q = static_cast<const uint8_t *>(q); a.q_ld = q_ld;
     a.s = scales; a.s_ld = s_ld; a.s_inc = s_inc;
     a.n = n; a.y = y; a.y_ld = y_ld;
+    if (!form) form = mm_form(a);
     unsigned *fault = cmolcu_fault_word(w->device);
     const cudaStream_t st = (cudaStream_t)stream;
     FP8_TRY(who, fp8_with_type(y_dtype, [&](auto t) {
-        return mm_pick<decltype(t)>(a, fault, st);
+        return mm_run<decltype(t)>(form, a, fault, st);
     }));
     return 0;
+}
+
+extern "C" int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld, const float *scales,
+                                 long long s_ld, long long s_inc, int n, void *y, int y_dtype, long long y_ld,
+                                 void *stream) {
+    return matmul("cmolcu_fp8_matmul", 0, w, q, q_ld, scales, s_ld, s_inc, n, y, y_dtype, y_ld, stream);
+}
+
+extern "C" int cmolcu_fp8_matmul_form(const cmolcu_fp8_weight_t *w, int n) {
+    if (!w || n < 1 || n > 1 << 30) return 0;
+    Fp8Device dev(w->device);
+    Fp8MmArgs a = {};
+    a.w = w->w;
+    a.n = n;
+    return mm_form(a);
+}
+
+extern "C" int cmolcu_fp8_matmul_as(int form, const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
+                                    const float *scales, long long s_ld, long long s_inc, int n, void *y, int y_dtype,
+                                    long long y_ld, void *stream) {
+    static const char *who = "cmolcu_fp8_matmul_as";
+    if (form != CMOLCU_FP8_FEW && form != 16 && form != 32 && form != 64 && form != 128 && form != 256) {
+        cmolcu_set_error("%s: no form %d", who, form);
+        return -1;
+    }
+    if (form == CMOLCU_FP8_FEW && n > 16) { cmolcu_set_error("%s: n=%d is too many for form %d", who, n, form); return -1; }
+    return matmul(who, form, w, q, q_ld, scales, s_ld, s_inc, n, y, y_dtype, y_ld, stream);
 }

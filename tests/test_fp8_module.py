@@ -64,3 +64,13 @@ def test_activations_that_require_a_gradient_are_refused():
         fp8.rmsnorm(x, gains)
     with pytest.raises(pkg.CmolError, match="wanted a GPU"):         # and so may a weight that is quantised
         fp8.Fp8Weight.quantize(torch.nn.Parameter(torch.zeros(2, 256)))
+
+
+def test_forms_of_the_product_are_refused_by_name():
+    L = pkg.lib()
+    P = 1 << 20
+    for form, n, says in [(0, 4, "no form 0"), (7, 4, "no form 7"), (512, 4, "no form 512"),
+                          (8, 17, "n=17 is too many for form 8"), (64, 4, "NULL argument"), (256, 4, "NULL argument")]:
+        assert L.cmolcu_fp8_matmul_as(form, None, P, 128, P, 1, 4, n, P, 0, 128, None) == -1
+        assert pkg.last_error() == f"cmolcu_fp8_matmul_as: {says}"
+    assert L.cmolcu_fp8_matmul_form(None, 4) == 0
