@@ -507,7 +507,7 @@ struct Fp8MmtArgs {
     CUtensorMap tm_y;          // where vy: y, in boxes of 64 bytes x 32 rows, 64-byte swizzle
     Fp8MmArgs   a;
     int         mt, rt;        // tiles of activation rows and of weight rows
-    int         vy;            // rows of y start on 16-byte boundaries
+    int         vy;            // rows of y start on 16-byte boundaries: copies write y
     unsigned   *fault;
 };
 
@@ -727,7 +727,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
             if (t + pairs < tiles) nx = tile(t + pairs);
             if (!ok || wrow >= w.rows) continue;
             // ---- out: 64 bytes of each of the warp's 32 rows at a time, through shared memory ----
+            // A copy out ends at y's last column only in whole 16 bytes (it wrote into what lies between the rows), so the
+            // last box goes value by value where the columns' bytes are not a multiple of that.
             constexpr int E = 64 / (int)sizeof(TY), V = 16 / (int)sizeof(TY);   // columns a pass, a 16-byte chunk
+            const int by_copy = !p.vy ? 0 : w.rows % V ? w.rows / E * E : w.rows;   // columns that copies write
 #pragma unroll
             for (int ps = 0; ps < R / E; ps++) {
                 uint8_t *const stg = out + flip * (32 * 64);
@@ -753,29 +756,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMT_THREADS, 1) k_fp
                     t5_fence_proxy();
                     __syncwarp();
                     if (lane == 0) {
-                        if (col0 < w.rows && row0 < p.a.n) t5_tma_store_2d(&p.tm_y, col0, (int)row0, stg);
+                        if (col0 < by_copy && row0 < p.a.n) t5_tma_store_2d(&p.tm_y, col0, (int)row0, stg);
                         t5_tma_store_commit();                            // one group a pass, as the wait counts them
                     }
-                } else {
-                    __syncwarp();
-                    // rows at any alignment: 32 consecutive values of a row an instruction (f32: two passes'), eight
-                    // rows in flight
-                    constexpr int PP = 32 / E;
-                    if (ps % PP == PP - 1) {
-                        const int c0 = col0 - (PP - 1) * E + lane, e = lane % E;
-                        const uint8_t *const src = PP == 1 ? stg : out + (lane / E) * (32 * 64);
-                        const int rows = c0 < w.rows ? (int)min((long long)32, p.a.n - row0) : 0;
-                        TY *y = static_cast<TY *>(p.a.y) + row0 * p.a.y_ld + c0;
-                        for (int b = 0; b < 32; b += 8) {
-                            TY v[8];
+                }
+                __syncwarp();
+                // the other columns: 32 consecutive values of a row an instruction (f32: two passes'), eight rows in
+                // flight
+                constexpr int PP = 32 / E;
+                if (by_copy < w.rows && ps % PP == PP - 1 && col0 + E > by_copy) {
+                    const int c0 = col0 - (PP - 1) * E + lane, e = lane % E;
+                    const uint8_t *const src = PP == 1 ? stg : out + (lane / E) * (32 * 64);
+                    const int rows = c0 >= by_copy && c0 < w.rows ? (int)min((long long)32, p.a.n - row0) : 0;
+                    TY *y = static_cast<TY *>(p.a.y) + row0 * p.a.y_ld + c0;
+                    for (int b = 0; b < 32; b += 8) {
+                        TY v[8];
 #pragma unroll
-                            for (int u = 0; u < 8; u++)
-                                v[u] = reinterpret_cast<const TY *>(src + mmt_place(b + u, e / V))[e % V];
+                        for (int u = 0; u < 8; u++)
+                            v[u] = reinterpret_cast<const TY *>(src + mmt_place(b + u, e / V))[e % V];
 #pragma unroll
-                            for (int u = 0; u < 8; u++) {
-                                if (b + u < rows) *y = v[u];
-                                y += p.a.y_ld;
-                            }
+                        for (int u = 0; u < 8; u++) {
+                            if (b + u < rows) *y = v[u];
+                            y += p.a.y_ld;
                         }
                     }
                     __syncwarp();
@@ -927,7 +929,8 @@ static bool w_map(CUtensorMap *m, const Fp8W &w, int rows) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// y, written in boxes of 64 bytes x 32 rows; what lies past it is left alone.
+// y, written in boxes of 64 bytes x 32 rows; rows past it are left alone, and columns in
+// whole 16 bytes.
 template <typename TY>
 static bool y_map(CUtensorMap *m, const Fp8MmArgs &a) {
     const encode_t enc = encode_fn();
