@@ -870,14 +870,18 @@ static cudaError_t mm_launch(void (*k)(P), dim3 grid, int threads, size_t smem, 
     return cudaLaunchKernelEx(&cfg, k, p);
 }
 
-template <int NG, typename TY>
-static cudaError_t few_launch(const Fp8MmArgs &a, cudaStream_t st) {
+// Warps that share a row group's k: 32 warps an SM (us at 1, 2, 4, 8, 16 warps a row group: 22016x2048 12.0, 12.5, 10.9,
+// 11.0, 15.8; 2048x11008 33.6, 16.7, 9.2, 5.3, 4.8; 49152x2048 21.6, 19.7, 19.5, 21.2, 33.1).
+static int few_split(const Fp8MmArgs &a) {
     const int groups = (a.w.rows + 15) / 16;
-    // 32 warps an SM (us at 1, 2, 4, 8, 16 warps a row group: 22016x2048 12.0, 12.5, 10.9, 11.0, 15.8; 2048x11008
-    // 33.6, 16.7, 9.2, 5.3, 4.8; 49152x2048 21.6, 19.7, 19.5, 21.2, 33.1)
     int kw = 1;
     while (kw < 16 && (long long)groups * kw < device_sm_count() * 32LL && kw * 2 <= a.w.kblocks) kw *= 2;
-    const int wc = few_warps(kw);
+    return kw;
+}
+
+template <int NG, typename TY>
+static cudaError_t few_launch(const Fp8MmArgs &a, cudaStream_t st) {
+    const int groups = (a.w.rows + 15) / 16, kw = few_split(a), wc = few_warps(kw);
     const dim3 grid((groups * kw + wc - 1) / wc), block(32 * wc);
     switch (kw) {
     case 1: return launch_k(k_fp8_mm_few<NG, 1, TY>, grid, block, 0, st, true, a);
@@ -966,36 +970,52 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     return launch_k(kern, dim3(2 * pairs), dim3(MMT_THREADS), Cfg::smem, st, true, p);
 }
 
-// Which form, by what it is estimated to take (us, from measurements with weights
-// in L2): a fixed part and a block of 128 along k times the blocks that the
-// busiest SM goes through in turn.
-//   k_fp8_mm_n, NT = 16 / 32 / 64:  3.5 (4.3 at two CTAs an SM) + 0.40 / 0.50 / 0.80 a block
-//   k_fp8_mm_t, N = 128 / 256:      3.3 + 0.25 / 0.47 a block, 0.5 / 1.5 a tile
-// Measured, for instance (32, 64 | 128, 256):
-//   64x2048x2048  6.1, 6.8 | 7.0, 11.2      64x22016x2048  18.7, 17.3 | 17.5, 21.5
-//   128x2048x11008  14.4, 14.2 | 23.4, 42.3   256x22016x2048  -, 42.2 | 18.3, 22.6
-//   512x2048x2048  -, 11.3 | 7.5, 11.6        2048x22016x2048  -, - | 100, 97
-// Up to 16 rows k_fp8_mm_few comes first: always up to 8 (8x2048x2048 2.0 against
-// 4.1, 8x22016x2048 11.5 against 10.7), beyond while the matrix is small, as it reads
-// the activations again for every 16 weight rows (16x5760x960 3.8 against 4.2,
-// 16x11008x2048 8.5 against 6.5).
+// Which form, by what it is estimated to take (us, fitted to 18 weights of 0.9 to 67 MB at 1
+// to 8192 rows, each call with another weight so that they come from memory):
+//   k_fp8_mm_few            1.4 + 0.5 a round of CTAs + the larger of 0.20 a MB of weights (0.34 beyond 8 rows, where
+//                           registers are spilled) and 1.0 (2.0) a block along k of a warp beyond the two in flight
+//   k_fp8_mm_n, 16 / 32 / 64   2.3 / 2.4 / 3.0, at two CTAs an SM 0.55 / 0.75 / 1.5 and with a split of k 1.05 / 1.15 /
+//                           1.3 more; 0.26 / 0.32 / 0.59 a block of 128 along k and 2.2 / 2.6 / 3.4 between rounds of
+//                           CTAs; 0.077 / 0.076 / 0.04 a MB of weights
+//   k_fp8_mm_t, 128 / 256   3.6 / 3.8; a round of tiles 0.245 / 0.485 a block of 128 along k where it is the only
+//                           one, else 0.27 / 0.49, and 0.85 / 1.6 more
+// Of 376 measured calls, 9 take a form that is more than 6 % slower than the best (26 % at 64x2049x8192); all lose 0.5 %
+// together, and 475 calls of other sizes 1.0 %.  Measured, for instance (few; 16, 32, 64; 128, 256):
+//   1x960x2560  2.1; 4.1, 4.3, 5.3; -        1x22016x2048  10.9; 10.1, 11.9, 14.5; -
+//   16x5760x960  4.5; 4.7, 5.0, 6.3; -       16x11008x2048  9.5; 7.5, 8.4, 11; -
+//   64x2048x2048  -; 5.5, 5.9, 7.3; 7.9, 12  128x2048x11008  -; 17, 12.6, 14.4; 24.6, 44
+//   256x22016x2048  -; 70, 43, 39; 18.6, 22  512x22016x2048  -; 134, 83, 65; 29.1, 30.8
+//   1024x22016x2048  -; 55, 51               8192x22016x2048  -; 401, 367
 static int mm_form(const Fp8MmArgs &a) {
-    if (a.n <= 8 || (a.n <= 16 && (long long)a.w.rows * a.w.k < 12 << 20)) return CMOLCU_FP8_FEW;
-    const int sms = device_sm_count(), nts[3] = {16, 32, 64};
-    const double per[3] = {0.40, 0.50, 0.80};
+    static const struct { int nt; double fixed, two, split, block, round, mb; } mmn[3] = {
+        {16, 2.3, 0.55, 1.05, 0.26, 2.2, 0.077}, {32, 2.4, 0.75, 1.15, 0.32, 2.6, 0.076}, {64, 3.0, 1.5, 1.3, 0.59, 3.4, 0.04}};
+    static const struct { int n; double fixed, one, more, tile; } mmt[2] = {{128, 3.6, 0.245, 0.27, 0.85},
+                                                                          {256, 3.8, 0.485, 0.49, 1.6}};
+    const int sms = device_sm_count(), kb = a.w.kblocks;
+    const double mb = 1e-6 * a.w.rows * a.w.k;
     double best = 1e30;
     int form = 0;
-    for (int i = 0; i < 3; i++) {
+    auto take = [&](int f, double t) {
+        if (t < best) { best = t; form = f; }
+    };
+    if (a.n <= 16) {
+        const int kw = few_split(a), wc = few_warps(kw), slots = kw > 8 ? sms : 2 * sms;
+        const int ctas = ((a.w.rows + 15) / 16 * kw + wc - 1) / wc;
+        const int chain = (kb + kw - 1) / kw - 2;
+        take(CMOLCU_FP8_FEW, 1.4 + 0.5 * ((ctas - 1) / slots + 1) +
+                                 (a.n <= 8 ? std::max(0.20 * mb, 1.0 * chain) : std::max(0.34 * mb, 2.0 * chain)));
+    }
+    for (const auto &f : mmn) {
         int kb_per;
-        const long long ks = mmn_split(a, nts[i], kb_per), ctas = ((a.n - 1) / nts[i] + 1) * (long long)a.w.rblocks * ks;
-        const double waves = (double)((ctas + 2 * sms - 1) / (2 * sms)), t = (ctas > sms ? 4.3 : 3.5) + waves * kb_per * per[i] + 2 * (waves - 1);
-        if (t < best) { best = t; form = nts[i]; }
+        const long long ks = mmn_split(a, f.nt, kb_per), ctas = ((a.n - 1) / f.nt + 1) * (long long)a.w.rblocks * ks;
+        const double rounds = (double)((ctas - 1) / (2 * sms) + 1);
+        take(f.nt, f.fixed + (ctas > sms ? f.two : 0) + (ks > 1 ? f.split : 0) + rounds * kb_per * f.block +
+                       (rounds - 1) * f.round + f.mb * mb);
     }
     const long long mt = (a.n - 1) / 256 + 1, pairs = std::max(1, sms / 2);
-    for (int n = 128; n <= 256; n += 128) {
-        const long long rounds = (mt * ((a.w.rows - 1) / n + 1) + pairs - 1) / pairs;
-        const double t = 3.3 + rounds * (n == 128 ? a.w.kblocks * 0.25 + 0.5 : a.w.kblocks * 0.47 + 1.5);
-        if (t < best) { best = t; form = n; }
+    for (const auto &f : mmt) {
+        const long long rounds = (mt * ((a.w.rows - 1) / f.n + 1) - 1) / pairs + 1;
+        take(f.n, f.fixed + rounds * (kb * (rounds == 1 ? f.one : f.more) + f.tile));
     }
     return form;
 }

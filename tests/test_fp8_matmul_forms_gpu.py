@@ -165,3 +165,17 @@ def test_the_choice_is_one_of_the_forms():
                 assert torch.equal(W.matmul(q, s), _run(f, W, q, s, torch.empty(n, rows, device="cuda")))
             chosen.add(f)
     assert chosen >= {8, 32, 128, 256}, chosen
+
+
+def test_the_choice_follows_the_measurements():
+    """Sizes at which one form is measured far ahead of the others, on the GPU that the estimates were fitted on."""
+    from libcmol_b200 import fp8, lib
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the estimates are for 148 SMs")
+    for n, rows, k, form in [(1, 960, 2560, 8), (4, 2048, 2048, 8), (16, 1536, 576, 8), (8, 32768, 512, 16),
+                             (16, 8192, 2048, 16), (64, 5760, 960, 16), (192, 960, 2560, 32), (96, 2048, 8192, 32),
+                             (64, 22016, 2048, 64), (256, 22016, 2048, 128), (777, 2049, 8192, 128),
+                             (1024, 22016, 2048, 256), (8192, 22016, 2048, 256), (2048, 2048, 11008, 256)]:
+        W = fp8.Fp8Weight.quantize(torch.ones(rows, k, device="cuda"))
+        assert lib().cmolcu_fp8_matmul_form(W.h, n) == form, (n, rows, k)
+        W.free()
