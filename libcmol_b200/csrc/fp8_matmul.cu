@@ -892,9 +892,13 @@ static cudaError_t few_launch(const Fp8MmArgs &a, cudaStream_t st) {
     }
 }
 
-// CTAs that share k and their blocks each.  Powers of two, and not more than fill
-// most of one wave at two an SM: clusters of six, or of sixteen, left SMs empty
-// (96x2048x11008 at 6: 17.5 us, at 4: 14.4; 16x2048x11008 at 16: 15.6, at 8: 7.3).
+// CTAs that share k and their blocks each: a power of two that does not more than fill
+// most of one wave at two an SM (96x2048x11008 at 6 CTAs 17.5 us, at 4 14.4; 16x2048x11008
+// at 16 15.6, at 8 7.3), less those that the rounding up of their blocks leaves without
+// any (12 blocks over 8: 6 CTAs of 2).  Giving all of the power of two CTAs one block
+// fewer or more measured no better (16 / 32 / 64 columns, us: 37x576x1536 3.8, 4.1, 4.7 against 3.6, 4.1,
+// 4.8; 64x960x2560 5.8, 4.9, 5.8 against 5.3, 5.0, 6.3; 24x2048x1152 5.2, 4.2, 5.0 against 4.1, 4.0,
+// 5.1).
 static int mmn_split(const Fp8MmArgs &a, int nt, int &kb_per) {
     const long long ctas = ((a.n - 1) / nt + 1) * (long long)a.w.rblocks, slots = device_sm_count() * 7LL / 4;
     int ks = 1;
