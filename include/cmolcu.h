@@ -159,7 +159,8 @@ void cmolcu_matmul_noalloc(float *out, const void *a, const float *b,
  * calling thread's current device is left as it was.  n = 0 does nothing.  The
  * same call gives the same bits; how a sum is split depends on the sizes, so a
  * row's last bits may differ between calls with different n.
- * Outputs must not overlap inputs, but for res_out = res. */
+ * Addresses are multiples of their elements' size.  Outputs must not overlap inputs, but
+ * for res_out = res. */
 #define CMOLCU_BF16 30
 
 /* h = x + res (h = x when res is NULL); res_out = h rounded to res_dtype;

@@ -22,6 +22,14 @@ __host__ __device__ inline int fp8_blocks(int k) { return (k - 1) / FP8_BLOCK + 
 // Bytes of an activation element, 0 for a type that the path does not take.
 inline int fp8_elem_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
 
+// Whether an address is no multiple of its elements' size (accesses there would fault);
+// sets the message.
+inline bool fp8_misaligned(const char *who, const void *p, int elem_bytes) {
+    if (reinterpret_cast<uintptr_t>(p) % elem_bytes == 0) return false;
+    cmolcu_set_error("%s: an address is no multiple of its element's size", who);
+    return true;
+}
+
 // Calls f with a value of the element type of tag `dt` (checked by the caller).
 template <typename F>
 auto fp8_with_type(int dt, F f) {

@@ -342,6 +342,7 @@ static int out_check(const char *who, int n, int k, void *q, long long q_ld, con
     }
     if (n == 0) return 0;
     if (!q || !s) { cmolcu_set_error("%s: NULL argument", who); return -1; }
+    if (fp8_misaligned(who, s, 4)) return -1;
     if ((reinterpret_cast<uintptr_t>(q) & 15) || (n > 1 && (q_ld < k || q_ld % 16))) {
         cmolcu_set_error("%s: q rows must start on 16-byte boundaries (q_ld=%lld)", who, q_ld);
         return -1;
@@ -368,6 +369,9 @@ extern "C" int cmolcu_fp8_rmsnorm(int device, const void *x, int x_dtype, long l
         cmolcu_set_error("%s: NULL argument", who);
         return -1;
     }
+    if (fp8_misaligned(who, x, xb) || fp8_misaligned(who, res, rb) || fp8_misaligned(who, res_out, rb) ||
+        fp8_misaligned(who, norm_w, 4))
+        return -1;
     if (res && n > 1 && res_out_ld < k) {
         cmolcu_set_error("%s: rows of the residual overlap (res_out_ld=%lld)", who, res_out_ld);
         return -1;
@@ -405,6 +409,7 @@ extern "C" int cmolcu_fp8_swiglu(int device, const void *gate, long long gate_ld
     if (!eb) { cmolcu_set_error("%s: unsupported dtype %d", who, dtype); return -1; }
     if (n == 0) return 0;
     if (!gate || !up) { cmolcu_set_error("%s: NULL argument", who); return -1; }
+    if (fp8_misaligned(who, gate, eb) || fp8_misaligned(who, up, eb)) return -1;
     Fp8Device dev(device);
     FP8_TRY(who, dev.err);
     Fp8ActArgs a = {};

@@ -1044,6 +1044,7 @@ static int matmul(const char *who, int form, const cmolcu_fp8_weight_t *w, const
     if (!fp8_elem_bytes(y_dtype)) { cmolcu_set_error("%s: unsupported dtype %d", who, y_dtype); return -1; }
     if (n == 0) return 0;
     if (!q || !scales || !y) { cmolcu_set_error("%s: NULL argument", who); return -1; }
+    if (fp8_misaligned(who, scales, 4) || fp8_misaligned(who, y, fp8_elem_bytes(y_dtype))) return -1;
     if (n == 1) {                                       // a single row has no stride
         q_ld = (w->w.k + 15) / 16 * 16;
         y_ld = (w->w.rows + 15LL) / 16 * 16;

@@ -150,6 +150,7 @@ extern "C" int cmolcu_fp8_weight_upload_dev(int device, const void *q, long long
     static const char *who = "cmolcu_fp8_weight_upload_dev";
     if (shape_check(who, q, rows, k, q_ld, out)) return -1;
     if (!scales) { cmolcu_set_error("%s: NULL argument", who); return -1; }
+    if (fp8_misaligned(who, scales, 4)) return -1;
     if ((reinterpret_cast<uintptr_t>(q) & 15) || q_ld % 16) {
         cmolcu_set_error("%s: rows must start on 16-byte boundaries (q_ld=%lld)", who, q_ld);
         return -1;
@@ -168,6 +169,7 @@ extern "C" int cmolcu_fp8_weight_quantize_dev(int device, const void *w, int dty
     if (shape_check(who, w, rows, k, ld, out)) return -1;
     const int eb = fp8_elem_bytes(dtype);
     if (!eb) { cmolcu_set_error("%s: unsupported dtype %d", who, dtype); return -1; }
+    if (fp8_misaligned(who, w, eb)) return -1;
     Fp8Device dev(device);
     FP8_TRY(who, dev.err);
     cmolcu_fp8_weight_t *h = nullptr;
@@ -186,6 +188,7 @@ extern "C" int cmolcu_fp8_weight_read_dev(const cmolcu_fp8_weight_t *h, void *q,
                                           void *stream) {
     static const char *who = "cmolcu_fp8_weight_read_dev";
     if (!h || !q || !scales) { cmolcu_set_error("%s: NULL argument", who); return -1; }
+    if (fp8_misaligned(who, scales, 4)) return -1;
     const Fp8W &w = h->w;
     if ((reinterpret_cast<uintptr_t>(q) & 15) || (w.rows > 1 && (q_ld < w.k || q_ld % 16))) {
         cmolcu_set_error("%s: rows must start on 16-byte boundaries (q_ld=%lld)", who, q_ld);
