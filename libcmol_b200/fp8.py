@@ -226,6 +226,16 @@ class Fp8Weight:
         self._set(h, rows, k, index)
         return self
 
+    # One owner of the memory: a weight does not change, so a copy is the weight itself.
+    def __copy__(self):
+        return self
+
+    def __deepcopy__(self, memo):
+        return self
+
+    def __reduce__(self):
+        raise CmolError("Fp8Weight: lies in a GPU's memory and cannot be pickled; read() gives its values")
+
     @property
     def nbytes(self) -> int:
         return lib().cmolcu_fp8_weight_bytes(self.h)

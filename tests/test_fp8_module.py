@@ -74,3 +74,26 @@ def test_forms_of_the_product_are_refused_by_name():
         assert L.cmolcu_fp8_matmul_as(form, None, P, 128, P, 1, 4, n, P, 0, 128, None) == -1
         assert pkg.last_error() == f"cmolcu_fp8_matmul_as: {says}"
     assert L.cmolcu_fp8_matmul_form(None, 4) == 0
+
+
+def test_copies_of_a_weight_are_the_weight(monkeypatch):
+    """A weight does not change, and its memory is given back once however it was copied."""
+    import copy
+    import pickle
+    freed = []
+
+    class Lib:
+        def cmolcu_fp8_weight_free(self, h):
+            freed.append(h)
+
+    monkeypatch.setattr(fp8, "lib", Lib)
+    W = fp8.Fp8Weight.__new__(fp8.Fp8Weight)
+    W._set(C.c_void_p(64), 2, 256, 0)
+    layer = {"w": W}
+    for other in (copy.copy(W), copy.deepcopy(W), copy.deepcopy(layer)["w"]):
+        assert other is W
+    with pytest.raises(pkg.CmolError, match="Fp8Weight: .* read"):
+        pickle.dumps(W)
+    other.free()
+    W.free()
+    assert len(freed) == 1
