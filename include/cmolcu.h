@@ -168,7 +168,8 @@ void cmolcu_matmul_noalloc(float *out, const void *a, const float *b,
  * v = h when norm_w is NULL; q and scales of v.
  * x, res, res_out: device rows of k values of CMOLCU_F32, _F16 or _BF16, x_ld
  * / res_ld / res_out_ld values apart.  norm_w: k f32 values.  res_out may be
- * res itself; both are NULL or neither.  Sums of squares are in f32. */
+ * res itself; both are NULL or neither.  Sums of squares are in f32: a row where one
+ * passes f32's largest number gives zeros. */
 int cmolcu_fp8_rmsnorm(int device, const void *x, int x_dtype, long long x_ld,
                        const void *res, long long res_ld, void *res_out, long long res_out_ld, int res_dtype,
                        const float *norm_w, float eps, int n, int k,
@@ -209,7 +210,8 @@ size_t cmolcu_fp8_weight_bytes(const cmolcu_fp8_weight_t *w);   /* values and sc
 /* y(c, r) = sum_b sx(c, b) * sw(r/128, b) * sum_{k in b} qx(c, k) * qw(r, k) for
  * n >= 1 activation rows: y is [n][rows] of y_dtype (CMOLCU_F32, _F16 or
  * _BF16), y_ld values apart.  Products and sums in f32, one rounding at the
- * end.  Waits inside the kernels are bounded: where one runs out y is invalid and the
+ * end.  sx * sw is formed first: where it lies below 2^-126 it adds an error of up to
+ * 2^-125 a block, where it passes f32's largest number y is infinite or NaN.  Waits inside the kernels are bounded: where one runs out y is invalid and the
  * device's fault word says so once the kernel has finished (cmolcu_fault_status). */
 int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
                       const float *scales, long long s_ld, long long s_inc, int n,
