@@ -144,8 +144,10 @@ void cmolcu_matmul_noalloc(float *out, const void *a, const float *b,
  * Activations have a block for every 128 consecutive values of a row, weights
  * one for every 128 x 128 (a last block may be shorter).  The quantisers set
  *   scale = max(amax / 448, 2^-126),   q = v / scale rounded to nearest even,
- * with both quotients in f32, so a block with a NaN gets a NaN scale and one with
- * an infinity an infinite scale (and zeros for its finite values).
+ * in f32 (amax times the rounded 1/448; the quotient rounded to f32 first): the bits that
+ * torch's division of f32 tensors by 448.0 and by the scale gives on a GPU.  A
+ * block with a NaN gets a NaN scale and one with an infinity an infinite scale
+ * (and zeros for its finite values).
  *
  * Activations on the device: q is [n][k] bytes, k a multiple of 16, rows q_ld
  * bytes apart; q starts on a 16-byte boundary and q_ld is a multiple of 16 (it

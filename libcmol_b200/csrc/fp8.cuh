@@ -4,7 +4,8 @@
 // A value v of a block is stored as q = rn_e4m3(v / s), s = max(amax / 448,
 // 2^-126), where amax is the block's largest magnitude: 448 is e4m3's largest
 // value, and the floor keeps 1 / s finite for blocks of zeros or of
-// subnormals.  Both quotients are f32's, rounded to nearest.  A NaN in a block
+// subnormals.  In f32: s is amax times the rounded 1 / 448, and the quotient is
+// rounded to nearest before its rounding to 8 bits.  A NaN in a block
 // makes its scale and its q NaN; an infinity makes the scale infinite, its own q
 // NaN and the finite values' q zero: every product with such a block is NaN, as it
 // is NaN or infinite without the rounding to 8 bits.
@@ -189,13 +190,11 @@ __device__ __forceinline__ float2 fp8_div2(float2 v, Fp8Inv i) {
     return fp8_fma2(v, make_float2(i.hi, i.hi), fp8_mul2(v, make_float2(i.lo, i.lo)));
 }
 
-// Scale of a block from its largest magnitude: amax / 448 rounded to nearest, after
-// Markstein (1990), by the remainder of a first quotient (exact down to the floor: 448 is
-// 7 * 2^6).
+// Scale of a block from its largest magnitude: by the rounded 1 / 448, as torch divides a
+// tensor on a GPU by a number, within 2^-23 of amax / 448.
 __device__ __forceinline__ float fp8_scale(float amax) {
-    const float inv = 1.f / 448.f, lo = 1.17549435e-38f, q = amax * inv;
-    const float s = fmaf(fmaf(q, 448.f, -amax), -inv, q);
-    return s < lo ? lo : amax <= 3.40282347e38f ? s : amax;      // infinite and NaN pass
+    const float s = amax * (1.f / 448.f), lo = 1.17549435e-38f;
+    return s < lo ? lo : s;           // infinite and NaN pass
 }
 
 // Two e4m3 values, the first in the low byte (round to nearest even; a NaN

@@ -1,6 +1,6 @@
-"""The quantisers' arithmetic, bit for bit: scale = max(amax / 448, 2^-126) and
-q = v / scale rounded to nearest even, both quotients rounded to f32 as IEEE
-division rounds them.  The wanted values come from the CPU's division.
+"""The quantisers' arithmetic, bit for bit: scale = max(amax * r, 2^-126) with r the f32 next to
+1 / 448, and q = v / scale rounded to nearest even after IEEE's rounding of the quotient
+to f32.  The wanted values come from the CPU, and from f32 torch operations on the GPU.
 
 A quotient whose distance from a midpoint of f32 is below 2^-45 of its size may
 fall on the other side (one in 2^20 values); to show in q it has to lie beside a
@@ -11,6 +11,7 @@ torch = pytest.importorskip("torch")
 
 F32, F16, BF16, E4M3 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
 LOWEST = 2.0 ** -126
+R = torch.tensor(1.0) / 448.0
 
 pytestmark = pytest.mark.gpu
 
@@ -38,7 +39,7 @@ def _want_rows(x):
     n, k = x.shape
     kb = -(-k // 128)
     b = torch.nn.functional.pad(x, (0, kb * 128 - k)).view(n, kb, 128)
-    s = (b.abs().amax(-1) / 448).clamp_min(LOWEST)
+    s = (b.abs().amax(-1) * R).clamp_min(LOWEST)
     return _quotients(b, s.unsqueeze(-1)).view(n, -1)[:, :k], s
 
 
@@ -77,7 +78,7 @@ def test_values_between_two_of_e4m3():
     g = torch.Generator().manual_seed(2)
     top = 448 * torch.exp2(torch.randint(-20, 20, (512, 1), generator=g).float()) * (
         1 + torch.randint(0, 1 << 10, (512, 1), generator=g).float() / (1 << 10))
-    s = top / 448
+    s = top * R
     grid = torch.arange(0, 127, dtype=torch.uint8).view(E4M3).float()
     mid = (grid[1:] + grid[:-1]) / 2
     v = s * mid[torch.randint(0, 126, (512, 126), generator=g)]
@@ -114,6 +115,18 @@ def test_weights(t):
     p = torch.zeros(rb * 128, kb * 128)
     p[:rows, :k] = w.float().cpu()
     p = p.view(rb, 128, kb, 128)
-    want = (p.abs().amax((1, 3)) / 448).clamp_min(LOWEST)
+    want = (p.abs().amax((1, 3)) * R).clamp_min(LOWEST)
     assert (s.cpu() == want).all()
     _same(q, _quotients(p, want[:, None, :, None]).reshape(rb * 128, kb * 128)[:rows, :k])
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_the_bits_of_torch_operations_on_the_gpu(t):
+    from libcmol_b200 import fp8
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(1000, 2560, generator=g, device="cuda").to(t)
+    q, s = fp8.quantize(x)
+    b = x.float().view(1000, 20, 128)
+    ws = (b.abs().amax(-1) / 448.0).clamp_min(LOWEST)
+    assert torch.equal(s, ws)
+    _same(q, (b / ws.unsqueeze(-1)).clamp(-448, 448).to(E4M3).view(1000, 2560).cpu())

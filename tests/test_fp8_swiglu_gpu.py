@@ -3,11 +3,10 @@ gate that is not zero in a block, the block's scale is |v| / 448 in f32.
 
 Bound, u = 2^-24.  Up to |gate| = 87: the power of two is within 2 units of its
 last place (4 u), 1 + exp(-gate) takes two roundings (2 u), the reciprocal is within
-one unit (2 u), the two products and the scale's quotient u each: 11 u, and 87 times the
-error of f32's ln(2) in the exponent, 2.8e-9: 4.1 u.
+one unit (2 u), the two products u each, the scale's product with 1/448 (off by 0.75 u)
+1.75 u: 11.75 u, and 87 times the error of f32's ln(2) in the exponent, 2.75e-9: 4.01 u.
 Below -87, v = gate * exp(gate/2) * up * exp(gate/2): two exponentials (2 units, 4 u each), three
-products and the scale's quotient: 12 u.  Terms of second order are far below one more u:
-16 u for both."""
+products and the scale's: 12.75 u.  Terms of second order are below 0.1 u: 16 u for both."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -107,7 +106,7 @@ def test_infinite_gates():
     gate[0, 5], gate[1, 5], gate[2, 5], gate[3, 5] = float("inf"), -float("inf"), 3e38, -3e38
     q, s = fp8.swiglu(gate, up)
     assert torch.isinf(s[0, 0]) and torch.isnan(q[0, 5].float()) and torch.isnan(s[1, 0])
-    assert s[2, 0] == torch.tensor(3e38) / 448 and s[3, 0] == LOWEST and (q[3].float() == 0).all()
+    assert s[2, 0].item() == (torch.tensor(3e38) * (torch.tensor(1.0) / 448)).item() and s[3, 0] == LOWEST and (q[3].float() == 0).all()
 
 
 @pytest.mark.parametrize("t", [F32, F16, BF16])
