@@ -225,7 +225,8 @@ int cmolcu_fp8_matmul(const cmolcu_fp8_weight_t *w, const void *q, long long q_l
  *   16, 32, 64      that many activation rows by 128 weight rows a CTA, k split over a
  *                   cluster where CTAs are few;
  *   128, 256        256 activation rows by that many weight rows a pair of CTAs.
- * _form says which one a call with n rows takes (0: n < 1 or no weight); _as runs a given one
+ * _form says which one a call with n rows takes, rows of y on 16-byte boundaries (0: n < 1 or
+ * no weight); _as runs a given one
  * (_FEW up to 16 rows, the others any n).  For tests and measurements: sums are split
  * differently, so last bits differ. */
 #define CMOLCU_FP8_FEW 8

@@ -963,7 +963,7 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
     if (!q_map(&p.tm_q, a, FP8_BLOCK) || !w_map(&p.tm_w, a.w, Cfg::rows)) return cudaErrorInvalidValue;
     p.mt = (a.n - 1) / 256 + 1;
     p.rt = (a.w.rows - 1) / N + 1;
-    p.vy = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.y_ld * sizeof(TY)) % 16 == 0;
+    p.vy = fp8_vec(a.y, a.y_ld * (long long)sizeof(TY)) > 0;
     if (p.vy && !y_map<TY>(&p.tm_y, a)) return cudaErrorInvalidValue;
     // the register split of the kernel adds up only to what it was built with
     static std::atomic<int> ready[64];
@@ -980,9 +980,10 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
 //                           registers are spilled) and 1.0 (2.0) a block along k of a warp beyond the two in flight
 //   k_fp8_mm_n, 16 / 32 / 64   2.3 / 2.4 / 3.0, at two CTAs an SM 0.55 / 0.75 / 1.5 and with a split of k 1.05 / 1.15 /
 //                           1.3 more; 0.26 / 0.32 / 0.59 a block of 128 along k and 2.2 / 2.6 / 3.4 between rounds of
-//                           CTAs; 0.077 / 0.076 / 0.04 a MB of weights
+//                           CTAs (f32 0.1 / 0.2 / 0.4 more); 0.077 / 0.076 / 0.04 a MB of weights
 //   k_fp8_mm_t, 128 / 256   3.6 / 3.8; a round of tiles 0.245 / 0.485 a block of 128 along k where it is the only
-//                           one, else 0.27 / 0.49, and 0.85 / 1.6 more
+//                           one, else 0.27 / 0.49, and 0.85 / 1.6 more; where rows of y do not start on 16-byte
+//                           boundaries 1.1 / 2.8 on top (f32 3.1 / 5.9), which hides from 4 blocks along k on
 // Of 376 measured calls, 9 take a form that is more than 6 % slower than the best (26 % at 64x2049x8192); all lose 0.5 %
 // together, and 475 calls of other sizes 1.0 %.  Measured, for instance (few; 16, 32, 64; 128, 256):
 //   1x960x2560  2.1; 4.1, 4.3, 5.3; -        1x22016x2048  10.9; 10.1, 11.9, 14.5; -
@@ -990,11 +991,12 @@ static cudaError_t mmt_launch(const Fp8MmArgs &a, unsigned *fault, cudaStream_t 
 //   64x2048x2048  -; 5.5, 5.9, 7.3; 7.9, 12  128x2048x11008  -; 17, 12.6, 14.4; 24.6, 44
 //   256x22016x2048  -; 70, 43, 39; 18.6, 22  512x22016x2048  -; 134, 83, 65; 29.1, 30.8
 //   1024x22016x2048  -; 55, 51               8192x22016x2048  -; 401, 367
-static int mm_form(const Fp8MmArgs &a) {
+//   4096x16383x128 bf16, y unaligned  -; -; 65, 72 (aligned 42, 31)
+static int mm_form(const Fp8MmArgs &a, bool aligned, int elem_bytes) {
     static const struct { int nt; double fixed, two, split, block, round, mb; } mmn[3] = {
         {16, 2.3, 0.55, 1.05, 0.26, 2.2, 0.077}, {32, 2.4, 0.75, 1.15, 0.32, 2.6, 0.076}, {64, 3.0, 1.5, 1.3, 0.59, 3.4, 0.04}};
-    static const struct { int n; double fixed, one, more, tile; } mmt[2] = {{128, 3.6, 0.245, 0.27, 0.85},
-                                                                          {256, 3.8, 0.485, 0.49, 1.6}};
+    static const struct { int n; double fixed, one, more, tile, out16, out32; } mmt[2] = {
+        {128, 3.6, 0.245, 0.27, 0.85, 1.1, 3.1}, {256, 3.8, 0.485, 0.49, 1.6, 2.8, 5.9}};
     const int sms = device_sm_count(), kb = a.w.kblocks;
     const double mb = 1e-6 * a.w.rows * a.w.k;
     double best = 1e30;
@@ -1013,13 +1015,15 @@ static int mm_form(const Fp8MmArgs &a) {
         int kb_per;
         const long long ks = mmn_split(a, f.nt, kb_per), ctas = ((a.n - 1) / f.nt + 1) * (long long)a.w.rblocks * ks;
         const double rounds = (double)((ctas - 1) / (2 * sms) + 1);
+        const double round = f.round + (elem_bytes == 4 ? 0.006 * f.nt : 0);
         take(f.nt, f.fixed + (ctas > sms ? f.two : 0) + (ks > 1 ? f.split : 0) + rounds * kb_per * f.block +
-                       (rounds - 1) * f.round + f.mb * mb);
+                       (rounds - 1) * round + f.mb * mb);
     }
     const long long mt = (a.n - 1) / 256 + 1, pairs = std::max(1, sms / 2);
     for (const auto &f : mmt) {
         const long long rounds = (mt * ((a.w.rows - 1) / f.n + 1) - 1) / pairs + 1;
-        take(f.n, f.fixed + rounds * (kb * (rounds == 1 ? f.one : f.more) + f.tile));
+        const double out = aligned ? 0 : (elem_bytes == 2 ? f.out16 : f.out32) * std::min(1.0, 4.0 / kb);
+        take(f.n, f.fixed + rounds * (kb * (rounds == 1 ? f.one : f.more) + f.tile + out));
     }
     return form;
 }
@@ -1061,7 +1065,8 @@ static int matmul(const char *who, int form, const cmolcu_fp8_weight_t *w, const
     a.q = static_cast<const uint8_t *>(q); a.q_ld = q_ld;
     a.s = scales; a.s_ld = s_ld; a.s_inc = s_inc;
     a.n = n; a.y = y; a.y_ld = y_ld;
-    if (!form) form = mm_form(a);
+    const int yb = fp8_elem_bytes(y_dtype);
+    if (!form) form = mm_form(a, fp8_vec(y, y_ld * yb) > 0, yb);
     unsigned *fault = cmolcu_fault_word(w->device);
     const cudaStream_t st = (cudaStream_t)stream;
     FP8_TRY(who, fp8_with_type(y_dtype, [&](auto t) {
@@ -1082,7 +1087,7 @@ extern "C" int cmolcu_fp8_matmul_form(const cmolcu_fp8_weight_t *w, int n) {
     Fp8MmArgs a = {};
     a.w = w->w;
     a.n = n;
-    return mm_form(a);
+    return mm_form(a, true, 4);
 }
 
 extern "C" int cmolcu_fp8_matmul_as(int form, const cmolcu_fp8_weight_t *w, const void *q, long long q_ld,
