@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(32 * norm_warps<TX, TR>(C)) k_fp8_norm(const F
     }
 }
 
-// Rows longer than a CTA's registers hold: one CTA a row, read twice.
+// Rows longer than a CTA's registers hold: one CTA a row, read twice (2048x20000 with the
+// residual: bf16 72 us, f32 112; 4.0 and 4.8 TB/s of the bytes counted once).
 template <typename TX, typename TR>
 __global__ void __launch_bounds__(512) k_fp8_norm_long(const Fp8ActArgs a) {
     using Row = NormRow<TX, TR, 1>;

@@ -36,10 +36,11 @@ struct Fp8MmArgs {
 // the operand of the warp-wide product m16n8k32: the order of k within a block is
 // the same permutation for both operands.  A block's product starts from zero and
 // is scaled and added in f32.  The KW warps of the same rows add up through shared
-// memory, in order.  4.8 us at 1x2048x11008 (4.7 TB/s), 10.9 at 1x22016x2048 (4.2).
-// (tcgen05 takes 128 rows at once, from shared memory: a ring,
-// 172 CTAs for 22016 rows on 148 SMs and a cluster's sum where rows are few; it
-// measured 11.3 us at 1x22016x2048 and 13.2 us at 1x2048x11008.)
+// memory, in order.  6.2 us at 1x2048x11008 with weights from memory (3.6 TB/s; 4.5 us
+// with the weight in L2), 2.1 at 1x960x2560.  k_fp8_mm_n with 16 columns takes 7.4 and 4.1
+// there, but 10.1 us at 1x22016x2048 against 10.8: warps of more rows than a wave holds start
+// their loads from nothing in every round.  Beyond 8 rows (two column groups) 100 to 204
+// bytes a thread spill at 128 registers.
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -154,7 +155,8 @@ __global__ void __launch_bounds__(32 * few_warps(KW), KW > 8 ? 1 : 2) k_fp8_mm_f
 // the summing warps' release of tensor memory, `done` is the product's commit.
 // Scales come eight blocks at a time.
 //
-// 8.6 us at 37x2048x11008 (eleven blocks a CTA), 17 at 64x22016x2048.
+// With weights from memory 9.3 us at 37x2048x11008 (eleven blocks a CTA; 8.6 with the weight
+// in L2), 9.7 at 1x22016x2048 (NT = 16, 4.6 TB/s), 16.2 at 64x22016x2048 (NT = 64).
 //
 // Warps: 0 loads, 1 and 2 products in turn (1 also tensor memory), 3 scales, 4-11
 // sums.
@@ -477,8 +479,8 @@ __global__ void __launch_bounds__(MMN_THREADS, 2) k_fp8_mm_n(const __grid_consta
 // part of tensor memory that the block will use, `done` (the products' commit,
 // in both CTAs) frees the stage and hands the sums their block.
 //
-// 354 to 393 us at 8192x22016x2048 from one GPU to another (1.9 to 2.1 PFLOP/s, the
-// tensor pipe half used): the summing warps take ~900 clocks a block of 256 columns,
+// 354 to 394 us at 8192x22016x2048 (N = 256) from one GPU to another (1.9 to 2.1 PFLOP/s, the
+// tensor pipe half used; N = 128 takes 401 to 423): the summing warps take ~900 clocks a block of 256 columns,
 // most of it waits for tensor memory one load after another.
 //
 // Warps: 0 loads, 1 and 3 products (rank 0), 2 tensor memory, 4-11 sums.
